@@ -290,6 +290,27 @@ int obman_adam_step(const obman_adam_tensor* tensors, int count, double lr, doub
                     double weight_decay, obman_stream_t stream);
 int obman_bf16_shadow(const float* src, uint16_t* dst, long n, obman_stream_t stream);
 
+/* ---- K16: the gradient norm over a list of tensors, clipping, and the clipped optimizer step -----
+ * norm = (sum |g|^p)^(1/p) over all elements of all tensors (norm: 2 = L2, 1 = L1, 0 = largest |g|); clipping multiplies every
+ * element by min(1, max_norm / (norm + 1e-6)) in fp32 and rounds once to the tensor's type (torch.nn.utils.clip_grad_norm_).
+ * g / n / type: HOST arrays of `count` device pointers, element counts and types (0 fp32, 1 bf16, 2 fp16); the elements of a
+ * tensor are contiguous from g[i] on, at element alignment.  Empty tensors and an empty list are allowed (norm 0).  Sums are
+ * fp64 in a fixed order: the same bits every call.  A NaN in any tensor gives a NaN norm and, as in torch, NaN gradients; an
+ * infinite norm multiplies by 0.  ws: obman_grad_norm_ws_doubles(count) doubles of scratch; out: one device float, the norm. */
+long obman_grad_norm_ws_doubles(int count);
+int obman_grad_norm(void* const* g, const long* n, const int* type, int count, int norm, double* ws, float* out, obman_stream_t stream);
+int obman_grad_clip(void* const* g, const long* n, const int* type, int count, int norm, float max_norm, double* ws, float* out,
+                    obman_stream_t stream);
+/* The optimizer step on clipped gradients without writing them: obman_adam_norm_partials sums the squares of every gradient of
+ * `n_lists` descriptor lists (the parameter groups) into ws and says how many doubles that were (*parts, HOST);
+ * obman_adam_step_clipped then is obman_adam_step on g * min(1, max_norm / (norm + 1e-6)).  clip: two device floats, the norm and the
+ * factor: written by the call that gets parts > 0, read by all (later groups pass parts = 0).  corr: 2 * count device floats of scratch. */
+int obman_adam_norm_partials(const obman_adam_tensor* const* lists, const int* counts, int n_lists, double* ws, int* parts,
+                             obman_stream_t stream);
+int obman_adam_step_clipped(const obman_adam_tensor* tensors, int count, double lr, double beta1, double beta2, double eps,
+                            double weight_decay, const double* partials, int parts, double max_norm, float* clip, float* corr,
+                            obman_stream_t stream);
+
 /* ---- K12: objpoints3d = scale * verts + trans ---------------------------------------------------
  * Replaces `scaled = scale.unsqueeze(1) * verts; points = scaled + trans.unsqueeze(1)` (atlasbranch.py:133-138) and its
  * autograd backward (two broadcast products and two [B,N,3] -> [B,1,.] reductions).  verts / out / g / gverts [B,N,3],

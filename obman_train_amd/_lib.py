@@ -9,7 +9,7 @@ import os
 from .build import LIB
 
 _c_void_p, _c_int, _c_long, _c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 # name -> (restype, argtypes); 'p' pointer, 'i' int, 'l' long, 'f' float
 _SIGNATURES = {
@@ -46,6 +46,11 @@ _SIGNATURES = {
     "obman_imgstream_ws_bytes": (_c_long, "iii"),
     "obman_imgstream_fwd": (_c_int, "piiip" "ii" "iii" "pp" "pp" "p"),
     "obman_adam_step": (_c_int, "pi" "ddddd" "p"),
+    "obman_grad_norm_ws_doubles": (_c_long, "i"),
+    "obman_grad_norm": (_c_int, "pppi" "i" "pp" "p"),
+    "obman_grad_clip": (_c_int, "pppi" "if" "pp" "p"),
+    "obman_adam_norm_partials": (_c_int, "ppi" "pp" "p"),
+    "obman_adam_step_clipped": (_c_int, "pi" "ddddd" "pid" "pp" "p"),
     "obman_bf16_shadow": (_c_int, "ppl" "p"),
     "obman_affine_points_fwd": (_c_int, "ppp" "ii" "p" "p"),
     "obman_affine_points_ws_floats": (_c_long, "i"),

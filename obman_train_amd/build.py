@@ -16,6 +16,10 @@ OBJ = os.path.join(CSRC, "build")
 LIB = os.path.join(CSRC, "libobman_hip.so")
 ARCH = "gfx950"
 FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function"]
+# no packed fp32 instructions (v_pk_add / mul / fma_f32), which hipcc -O3 makes of ordinary float code by itself: some of their forms
+# have given wrong results on this hardware now and then.  Element-wise the scalar forms round identically.  (hipcc's host pass says
+# that it does not know the feature: harmless.)
+FLAGS += ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # measurement builds only (e.g. OBMAN_EXTRA_HIPCC_FLAGS=-DOBMAN_F2_TIMING with --force): never set for the product library
 FLAGS += os.environ.get("OBMAN_EXTRA_HIPCC_FLAGS", "").split()
 

@@ -11,12 +11,13 @@
 //   K14 obman_gt_object_stats    centroid, centred cloud and max point norm of the ground-truth object points
 //                                (atlasbranch.py:211-222: gt.mean(1), gt - centroid, norm(.,2,2).max(1))
 #include "common.h"
+#include "gradnorm.h"
 #include "../../include/obman_hip.h"
 
 namespace {
 
 // ------------------------------------------------------------------------------------------------------------------ K11 Adam
-constexpr int ADAM_MAX = 64;        // tensors per launch: 64 x 52 bytes of kernel arguments (limit 4 KB)
+constexpr int ADAM_MAX = 64;        // tensors per launch: 64 x 60 bytes of kernel arguments (limit 4 KB)
 constexpr int ADAM_CHUNK = 4096;    // elements per block: 256 threads x 4 float4
 struct AdamBatch {
   float* p[ADAM_MAX];
@@ -29,7 +30,7 @@ struct AdamBatch {
   int first_block[ADAM_MAX + 1];  // prefix of the per-tensor block counts
   int count;
 };
-static_assert(sizeof(AdamBatch) <= 4096, "kernel argument block");
+static_assert(sizeof(AdamBatch) <= 4096 - 64, "kernel argument block");
 
 __global__ void adam_tick_kernel(AdamBatch b) {
   const int t = threadIdx.x;
@@ -56,7 +57,11 @@ __device__ __forceinline__ void adam_one(float& p, float g, float& m, float& v, 
 
 // lr, beta1, beta2 arrive as DOUBLES (what torch.optim.Adam holds): 1 - beta2 formed in fp32 from the rounded 0.999f is 1.3e-5 off
 // the 0.001 every torch implementation multiplies by (first version: exp_avg_sq drifted from torch's by exactly that factor)
-__global__ __launch_bounds__(256) void adam_kernel(AdamBatch b, double lr, double beta1, double beta2, float eps, float wd) {
+// CLIP: the gradients are multiplied by clip[1] on their way in (they are not written back), and what depends on a tensor's step
+// count comes from adam_clip_kernel instead of two fp64 powers per thread
+template <bool CLIP>
+__global__ __launch_bounds__(256) void adam_kernel(AdamBatch b, double lr, double beta1, double beta2, float eps, float wd,
+                                                  const float* __restrict__ clip, const float2* __restrict__ corr) {
   // which tensor: binary search of the block id in the (scalar) prefix table
   int lo = 0, hi = b.count;
   while (hi - lo > 1) {
@@ -70,10 +75,17 @@ __global__ __launch_bounds__(256) void adam_kernel(AdamBatch b, double lr, doubl
   float* __restrict__ m = b.m[t];
   float* __restrict__ v = b.v[t];
   unsigned short* __restrict__ sh = b.shadow[t];
-  const double step = (double)*b.step[t];  // already incremented by adam_tick_kernel
   AdamK k;
-  k.lr_over_bc1 = (float)(lr / (1.0 - pow(beta1, step)));
-  k.bc2_sqrt = (float)sqrt(1.0 - pow(beta2, step));
+  float gk = 1.f;
+  if constexpr (CLIP) {
+    gk = clip[1];
+    k.lr_over_bc1 = corr[t].x;
+    k.bc2_sqrt = corr[t].y;
+  } else {
+    const double step = (double)*b.step[t];  // already incremented by adam_tick_kernel
+    k.lr_over_bc1 = (float)(lr / (1.0 - pow(beta1, step)));
+    k.bc2_sqrt = (float)sqrt(1.0 - pow(beta2, step));
+  }
   k.beta1w = (float)(1.0 - beta1); k.beta2 = (float)beta2; k.beta2w = (float)(1.0 - beta2); k.eps = eps; k.wd = wd;
   const bool vec = ((reinterpret_cast<size_t>(p) | reinterpret_cast<size_t>(g) | reinterpret_cast<size_t>(m) | reinterpret_cast<size_t>(v)) & 15) == 0 &&
                    (reinterpret_cast<size_t>(sh) & 7) == 0;
@@ -83,7 +95,8 @@ __global__ __launch_bounds__(256) void adam_kernel(AdamBatch b, double lr, doubl
     if (i >= n) break;
     if (vec && i + 4 <= n) {
       float4 P = *reinterpret_cast<const float4*>(p + i), M = *reinterpret_cast<const float4*>(m + i), V = *reinterpret_cast<const float4*>(v + i);
-      const float4 G = *reinterpret_cast<const float4*>(g + i);
+      float4 G = *reinterpret_cast<const float4*>(g + i);
+      if constexpr (CLIP) { G.x *= gk; G.y *= gk; G.z *= gk; G.w *= gk; }
       adam_one(P.x, G.x, M.x, V.x, k); adam_one(P.y, G.y, M.y, V.y, k); adam_one(P.z, G.z, M.z, V.z, k); adam_one(P.w, G.w, M.w, V.w, k);
       *reinterpret_cast<float4*>(p + i) = P; *reinterpret_cast<float4*>(m + i) = M; *reinterpret_cast<float4*>(v + i) = V;
       if (sh) {
@@ -95,11 +108,32 @@ __global__ __launch_bounds__(256) void adam_kernel(AdamBatch b, double lr, doubl
     } else {
       for (long j = i; j < n && j < i + 4; ++j) {
         float P = p[j], M = m[j], V = v[j];
-        adam_one(P, g[j], M, V, k);
+        adam_one(P, CLIP ? g[j] * gk : g[j], M, V, k);
         p[j] = P; m[j] = M; v[j] = V;
         if (sh) sh[j] = bf16_rne(P);
       }
     }
+  }
+}
+
+// Before the clipped update: joins the block sums of the gradient norm (parts > 0; clip[0] = norm, clip[1] = factor), counts the steps and
+// forms what depends on them.  One block; 320 step pointers a launch.
+constexpr int ADAM_STEPS = 320;
+struct AdamSteps {
+  float* step[ADAM_STEPS];
+  int count;
+};
+__global__ __launch_bounds__(ADAM_STEPS) void adam_clip_kernel(AdamSteps s, double lr, double beta1, double beta2, const double* __restrict__ part, int parts,
+                                                              float max_norm, float* __restrict__ clip, float2* __restrict__ corr) {
+  const int t = threadIdx.x;
+  if (t < s.count) {
+    const float n = *s.step[t] + 1.f;
+    *s.step[t] = n;
+    corr[t] = make_float2((float)(lr / (1.0 - pow(beta1, (double)n))), (float)sqrt(1.0 - pow(beta2, (double)n)));
+  }
+  if (parts > 0) {
+    const float n32 = (float)gn::join<ADAM_STEPS>(part, parts, gn::NORM_2);
+    if (t == 0) { clip[0] = n32; clip[1] = gn::clip_factor(n32, max_norm); }
   }
 }
 
@@ -255,10 +289,8 @@ __global__ __launch_bounds__(256) void gt_stats_kernel(const float* __restrict__
 
 extern "C" {
 
-int obman_adam_step(const obman_adam_tensor* tensors, int count, double lr, double beta1, double beta2, double eps,
-                    double weight_decay, obman_stream_t stream) {
-  if (count < 0 || (count > 0 && !tensors)) return -1;
-  hipStream_t st = (hipStream_t)stream;
+static int adam_launch(const obman_adam_tensor* tensors, int count, double lr, double beta1, double beta2, double eps, double weight_decay,
+                       const float* clip, const float2* corr, hipStream_t st) {
   for (int base = 0; base < count; base += ADAM_MAX) {
     AdamBatch b;
     b.count = count - base < ADAM_MAX ? count - base : ADAM_MAX;
@@ -272,14 +304,58 @@ int obman_adam_step(const obman_adam_tensor* tensors, int count, double lr, doub
     }
     for (int i = b.count; i <= ADAM_MAX; ++i) b.first_block[i] = blocks;
     for (int i = b.count; i < ADAM_MAX; ++i) { b.p[i] = nullptr; b.g[i] = nullptr; b.m[i] = nullptr; b.v[i] = nullptr; b.shadow[i] = nullptr; b.step[i] = nullptr; b.n[i] = 0; }
-    adam_tick_kernel<<<1, ADAM_MAX, 0, st>>>(b);
-    OBMAN_LAUNCH_CHECK();
+    if (!clip) {
+      adam_tick_kernel<<<1, ADAM_MAX, 0, st>>>(b);
+      OBMAN_LAUNCH_CHECK();
+    }
     if (blocks > 0) {
-      adam_kernel<<<blocks, 256, 0, st>>>(b, lr, beta1, beta2, (float)eps, (float)weight_decay);
+      if (clip) adam_kernel<true><<<blocks, 256, 0, st>>>(b, lr, beta1, beta2, (float)eps, (float)weight_decay, clip, corr + base);
+      else adam_kernel<false><<<blocks, 256, 0, st>>>(b, lr, beta1, beta2, (float)eps, (float)weight_decay, nullptr, nullptr);
       OBMAN_LAUNCH_CHECK();
     }
   }
   return 0;
+}
+
+int obman_adam_step(const obman_adam_tensor* tensors, int count, double lr, double beta1, double beta2, double eps,
+                    double weight_decay, obman_stream_t stream) {
+  if (count < 0 || (count > 0 && !tensors)) return -1;
+  return adam_launch(tensors, count, lr, beta1, beta2, eps, weight_decay, nullptr, nullptr, (hipStream_t)stream);
+}
+
+int obman_adam_norm_partials(const obman_adam_tensor* const* lists, const int* counts, int n_lists, double* ws, int* parts, obman_stream_t stream) {
+  if (n_lists < 0 || (n_lists && (!lists || !counts)) || !ws || !parts) return -1;
+  int count = 0;
+  for (int l = 0; l < n_lists; ++l) {
+    if (counts[l] < 0 || (counts[l] && !lists[l])) return -1;
+    count += counts[l];
+  }
+  int l = 0, first = 0;  // tables are filled in index order: the list that holds tensor i is the current one or a later one
+  const auto get = [&](int i) {
+    while (i - first >= counts[l]) first += counts[l++];
+    const obman_adam_tensor& t = lists[l][i - first];
+    return gn::Item{const_cast<float*>(t.g), t.n, gn::F32};
+  };
+  return gn::partials(get, count, gn::NORM_2, ws, parts, (hipStream_t)stream);
+}
+
+int obman_adam_step_clipped(const obman_adam_tensor* tensors, int count, double lr, double beta1, double beta2, double eps, double weight_decay,
+                            const double* partials, int parts, double max_norm, float* clip, float* corr, obman_stream_t stream) {
+  if (count <= 0 || !tensors || parts < 0 || (parts && !partials) || !(max_norm >= 0.0) || !clip || !corr) return -1;
+  hipStream_t st = (hipStream_t)stream;
+  for (int base = 0; base < count; base += ADAM_STEPS) {
+    AdamSteps s;
+    s.count = count - base < ADAM_STEPS ? count - base : ADAM_STEPS;
+    for (int i = 0; i < s.count; ++i) {
+      if (!tensors[base + i].step) return -2;
+      s.step[i] = tensors[base + i].step;
+    }
+    for (int i = s.count; i < ADAM_STEPS; ++i) s.step[i] = nullptr;
+    adam_clip_kernel<<<1, ADAM_STEPS, 0, st>>>(s, lr, beta1, beta2, partials, base ? 0 : parts, (float)max_norm, clip,
+                                               reinterpret_cast<float2*>(corr) + base);
+    OBMAN_LAUNCH_CHECK();
+  }
+  return adam_launch(tensors, count, lr, beta1, beta2, eps, weight_decay, clip, reinterpret_cast<const float2*>(corr), st);
 }
 
 int obman_bf16_shadow(const float* src, uint16_t* dst, long n, obman_stream_t stream) {

@@ -13,6 +13,7 @@ import os
 import numpy as np
 import torch
 
+from obman_train_amd import optim
 from obman_train_amd.evaluation.evalutils import AverageMeters
 from obman_train_amd.evaluation.zimeval import EvalUtil
 from obman_train_amd.netscripts import savemano
@@ -21,7 +22,7 @@ from obman_train_amd.queries import TransQueries
 
 def epoch_pass(loader, model, epoch, optimizer=None, debug=True, freeze_batchnorm=False, display=False, display_freq=10,
                save_path="checkpoints/debug", idxs=None, train=True, inspect_weights=False, fig=None, save_results=False,
-               buckets=None, log_freq=1, verbose=False):
+               buckets=None, log_freq=1, verbose=False, max_grad_norm=None):
     avg_meters, time_meters = AverageMeters(), AverageMeters()
     if train:
         model.eval() if freeze_batchnorm else model.train()
@@ -44,6 +45,8 @@ def epoch_pass(loader, model, epoch, optimizer=None, debug=True, freeze_batchnor
             model_loss.backward()
             if buckets is not None:
                 buckets.finish()
+            if max_grad_norm is not None:  # all gradients together, by their global L2 norm
+                optim.clip_grad_norm_([p for g in optimizer.param_groups for p in g["params"]], max_grad_norm)
             optimizer.step()
         if save_results:  # epochpass3d.py:135-139: save_results/<train|val>/epoch_N/batch_XXXXXX.pkl
             split = "train" if train else "val"

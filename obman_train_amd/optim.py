@@ -9,20 +9,128 @@ other), with ``step()`` replaced:
   over the 350 MB it touches; this kernel streams 16-byte vectors of p, g, m, v);
 * the per-parameter step counters live on the device (one fp32 array), so the step records into a hipGraph like torch's
   ``capturable=True`` form, without its per-step host work;
+* ``max_grad_norm`` clips all gradients of all groups together by their global L2 norm (``clip_grad_norm_``'s rule) inside the
+  same kernel: the norm is one pass over the gradients, the clipped values are never written (``grad_norm`` holds the norm);
 * a parameter that carries a bf16 SHADOW (``attach_bf16_shadows``: the filters of a bf16-autocast encoder) gets
   ``shadow = bf16(p_new)`` written by the same kernel - the autocast encoder then reads the shadow
   (``ops.shadow_conv2d``) instead of launching one cast kernel per filter and step.
 No CPU path: parameters must be fp32 ROCm tensors (``trainer.make_optimizer`` only builds this optimizer for such models).
+
+``grad_norm`` and ``clip_grad_norm_`` are the same norm and clipping for any other optimizer (``csrc/gradnorm.hip``): lists of
+fp32 / bf16 / fp16 gradients of any sizes, one or two launches per 192 tensors.
 """
 import ctypes
+from array import array
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib, ops
 
+_GRAD_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_NORMS = {2.0: 2, 1.0: 1, float("inf"): 0}
+
+
+def _norm_kind(norm_type):
+    kind = _NORMS.get(float(norm_type))
+    if kind is None:
+        raise ValueError("norm_type must be 1, 2 or inf, got %r" % (norm_type,))
+    return kind
+
+
+def _same_device(tensors, what):
+    """One device, strided fp32 / bf16 / fp16 tensors, or an error.  (One grouping call instead of a walk in Python: 92 gradients cost
+    6 us instead of 40, next to a kernel of 12.)"""
+    groups = list(torch._C._group_tensors_by_device_and_dtype([tensors], False))
+    dev = groups[0][0]
+    for d, dtype in groups:
+        if d.type != "cuda":
+            raise _lib.ObmanHipError("%s must be ROCm device tensors (the HIP path has no CPU fallback)" % what)
+        if dtype not in _GRAD_TYPES:
+            raise TypeError("%s must be fp32, bf16 or fp16, got %s" % (what, dtype))
+        if d != dev:
+            raise ValueError("%s must be on one device, got %s and %s" % (what, dev, d))
+    if any(t.layout != torch.strided for t in tensors):
+        raise TypeError("%s must be dense tensors" % what)
+    return dev, _GRAD_TYPES[groups[0][1]] if len(groups) == 1 else None
+
+
+def _norm_call(tensors, dev, one_type, norm_kind, max_norm=None):
+    """One C-ABI call over dense tensors of one device: -> the norm, a 0-dim fp32 tensor on that device."""
+    n = len(tensors)
+    ptrs = array("Q", map(torch.Tensor.data_ptr, tensors))
+    counts = array("q", map(torch.Tensor.numel, tensors))
+    types = array("i", [_GRAD_TYPES[t.dtype] for t in tensors] if one_type is None else [one_type]) * (1 if one_type is None else n)
+    with torch.cuda.device(dev):  # the launch goes to the tensors' device, on its current stream
+        out = torch.empty((), dtype=torch.float32, device=dev)
+        lib = _lib.lib()
+        ws = torch.empty(lib.obman_grad_norm_ws_doubles(n), dtype=torch.float64, device=dev)  # of this call alone: recorded into a graph it is the graph's
+        at = (ptrs.buffer_info()[0], counts.buffer_info()[0], types.buffer_info()[0])
+        if max_norm is None:
+            _lib.check(lib.obman_grad_norm(*at, n, norm_kind, ws.data_ptr(), out.data_ptr(), ops._stream()), "obman_grad_norm")
+        else:
+            _lib.check(lib.obman_grad_clip(*at, n, norm_kind, max_norm, ws.data_ptr(), out.data_ptr(), ops._stream()), "obman_grad_clip")
+    return out
+
+
+@torch.no_grad()
+def grad_norm(tensors, norm_type=2.0):
+    """The norm of all elements of all ``tensors`` (gradients, fp32 / bf16 / fp16, mixed) as one vector: a 0-dim fp32 tensor on
+    their device, without a host synchronisation.  ``norm_type`` 2, 1 or inf.  Summed in 64 bits in a fixed order: bit-reproducible.
+    An empty list gives 0 (on the CPU); entries that are ``None`` (parameters without a gradient) are skipped."""
+    kind = _norm_kind(norm_type)
+    if isinstance(tensors, torch.Tensor):
+        tensors = [tensors]
+    tensors = [t for t in tensors if t is not None]
+    if not tensors:
+        return torch.zeros(())
+    dev, one_type = _same_device(tensors, "tensors")
+    return _norm_call([t if ops._is_dense(t) else t.contiguous() for t in tensors], dev, one_type, kind)
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """``torch.nn.utils.clip_grad_norm_`` on this package's kernels: every gradient of ``parameters`` is multiplied in place by
+    ``min(1, max_norm / (norm + 1e-6))`` and the norm before clipping is returned (0-dim fp32 device tensor; nothing waits for it).
+
+    A parameter listed twice, or two that share one gradient tensor, is counted and scaled once.  As in torch, a NaN norm makes the
+    gradients NaN and an infinite one multiplies them by 0; ``error_if_nonfinite`` raises instead, before anything is scaled - it has
+    to wait for the device and cannot be recorded into a graph.  ``ObmanAdam(max_grad_norm=...)`` does the same without writing the
+    clipped gradients."""
+    kind = _norm_kind(norm_type)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError("max_norm must not be negative or NaN, got %r" % (max_norm,))
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = list({id(g): g for g in (p.grad for p in parameters) if g is not None}.values())
+    if not grads:
+        return torch.zeros(())
+    dev, one_type = _same_device(grads, "gradients")
+    odd = [i for i, g in enumerate(grads) if not ops._is_dense(g)]
+    for i in odd:
+        if torch._debug_has_internal_overlap(grads[i]) == 1:
+            raise ValueError("a gradient whose elements share memory (an expanded tensor) cannot be scaled in place")
+    if error_if_nonfinite:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("clip_grad_norm_(error_if_nonfinite=True) reads the norm on the host: it cannot be recorded into a graph")
+        norm = grad_norm(grads, norm_type)
+        if not torch.isfinite(norm):
+            raise RuntimeError("the total norm of order %s for gradients is non-finite, so it cannot be clipped" % (float(norm_type),))
+    work = list(grads)
+    for i in odd:
+        work[i] = grads[i].contiguous()
+    norm = _norm_call(work, dev, one_type, kind, max_norm)
+    for i in odd:
+        grads[i].copy_(work[i])
+    increment_version(grads)
+    return norm
+
 
 class ObmanAdam(torch.optim.Adam):
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, amsgrad=False, **kw):
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, amsgrad=False, max_grad_norm=None, **kw):
+        if max_grad_norm is not None and not float(max_grad_norm) >= 0.0:
+            raise ValueError("max_grad_norm must not be negative or NaN, got %r" % (max_grad_norm,))
         if amsgrad or kw.get("maximize"):
             raise ValueError("ObmanAdam implements plain Adam (traineval.py:112-116): no amsgrad / maximize")
         kw.pop("fused", None)
@@ -30,6 +138,8 @@ class ObmanAdam(torch.optim.Adam):
         kw.pop("foreach", None)
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=False, foreach=False, fused=False,
                          capturable=True)  # capturable: ``step`` entries are device tensors, as this kernel keeps them
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)  # read by every step; None = no clipping
+        self.grad_norm = None  # 0-dim fp32 device tensor: the L2 norm of the last clipped step's gradients, before clipping
         for group in self.param_groups:
             for p in group["params"]:
                 if not p.is_cuda or p.dtype != torch.float32:
@@ -51,6 +161,7 @@ class ObmanAdam(torch.optim.Adam):
                 loss = closure()
         lib = _lib.lib()
         stream = ops._stream()
+        work = []
         for gi, group in enumerate(self.param_groups):
             params = [p for p in group["params"] if p.grad is not None]
             if not params:
@@ -65,9 +176,35 @@ class ObmanAdam(torch.optim.Adam):
             lr = group["lr"]
             if torch.is_tensor(lr):
                 lr = float(lr)
-            _lib.check(lib.obman_adam_step(cache["addr"], len(params), float(lr), float(b1), float(b2), float(group["eps"]),
-                                           float(group["weight_decay"]), stream), "obman_adam_step")
+            work.append((cache["addr"], len(params), float(lr), float(b1), float(b2), float(group["eps"]), float(group["weight_decay"])))
+        if self.max_grad_norm is not None:
+            self._clipped(lib, work, stream)
+            return loss
+        for args in work:
+            _lib.check(lib.obman_adam_step(*args, stream), "obman_adam_step")
         return loss
+
+    def _clipped(self, lib, work, stream):
+        """The norm over every group's gradients, then each group's update on the clipped values.  Scratch of this call alone: recorded
+        into a graph it belongs to the graph, and two graphs of one optimizer share nothing but the parameters."""
+        if not work:
+            return
+        dev = next(p for g in self.param_groups for p in g["params"] if p.grad is not None).device
+        lists = (ctypes.c_void_p * len(work))(*[w[0] for w in work])
+        counts = (ctypes.c_int * len(work))(*[w[1] for w in work])
+        total = sum(w[1] for w in work)
+        ws = torch.empty(lib.obman_grad_norm_ws_doubles(total), dtype=torch.float64, device=dev)
+        corr = torch.empty(2 * max(w[1] for w in work), dtype=torch.float32, device=dev)
+        clip = torch.empty(2, dtype=torch.float32, device=dev)
+        parts = ctypes.c_int(0)
+        _lib.check(lib.obman_adam_norm_partials(ctypes.addressof(lists), ctypes.addressof(counts), len(work), ws.data_ptr(),
+                                                ctypes.addressof(parts), stream), "obman_adam_norm_partials")
+        first = parts.value
+        for args in work:
+            _lib.check(lib.obman_adam_step_clipped(*args, ws.data_ptr(), first, self.max_grad_norm, clip.data_ptr(), corr.data_ptr(), stream),
+                       "obman_adam_step_clipped")
+            first = 0
+        self.grad_norm = clip[0]
 
     def _build(self, params):
         """The launch's descriptor table (host array of device pointers) for this set of parameters; everything but the gradient

@@ -5,7 +5,9 @@ loss values stay on the device; ``read_losses`` batches them into one transfer w
 import torch
 
 
-def train_step(model, optimizer, sample, buckets=None):
+def train_step(model, optimizer, sample, buckets=None, max_grad_norm=None):
+    """``max_grad_norm``: clip the (averaged) gradients by their global L2 norm before the step, for any optimizer on a ROCm model
+    (``optim.clip_grad_norm_``); ``make_optimizer(..., max_grad_norm=...)`` does it inside the optimizer kernel instead."""
     total, results, losses = model.forward(sample)
     if buckets is not None and buckets.enabled:
         buckets.zero_grad()  # gradients are views into the all-reduce buckets: zero them in place
@@ -14,6 +16,10 @@ def train_step(model, optimizer, sample, buckets=None):
     total.backward()
     if buckets is not None:
         buckets.finish()
+    if max_grad_norm is not None:
+        from . import optim
+
+        optim.clip_grad_norm_([p for g in optimizer.param_groups for p in g["params"]], max_grad_norm)
     optimizer.step()
     return total, results, losses
 
@@ -27,9 +33,11 @@ def read_losses(losses):
     return dict(zip(keys, flat))
 
 
-def make_optimizer(model, name="adam", lr=1e-4, momentum=0.9, weight_decay=0.0, capturable=False):
+def make_optimizer(model, name="adam", lr=1e-4, momentum=0.9, weight_decay=0.0, capturable=False, max_grad_norm=None):
     """traineval.py:112-127 (defaults nets3dopts.py:249-273).  ``capturable``: the step may be recorded into a hipGraph
-    (``GraphedTrainStep``): Adam keeps its step counters on the device and never reads them on the host."""
+    (``GraphedTrainStep``): Adam keeps its step counters on the device and never reads them on the host.
+    ``max_grad_norm``: every step clips the gradients by their global L2 norm first, inside the optimizer kernel (adam on a ROCm
+    model only; other optimizers: ``train_step(..., max_grad_norm=...)``)."""
     params = [p for p in model.parameters() if p.requires_grad]
     if name == "adam":
         if params and all(p.is_cuda and p.dtype == torch.float32 for p in params):
@@ -41,8 +49,12 @@ def make_optimizer(model, name="adam", lr=1e-4, momentum=0.9, weight_decay=0.0, 
             base = getattr(model, "base_net", None)
             if base is not None and getattr(base, "autocast_dtype", None) == torch.bfloat16:
                 optim.attach_bf16_shadows(base)
-            return optim.ObmanAdam(params, lr=lr, weight_decay=weight_decay)
+            return optim.ObmanAdam(params, lr=lr, weight_decay=weight_decay, max_grad_norm=max_grad_norm)
+        if max_grad_norm is not None:
+            raise ValueError("make_optimizer(max_grad_norm=...) needs fp32 ROCm parameters: there is no CPU path")
         return torch.optim.Adam(params, lr=lr, weight_decay=weight_decay)
+    if max_grad_norm is not None:
+        raise ValueError("make_optimizer(max_grad_norm=...) is the adam kernel's; with %r pass max_grad_norm to train_step / epoch_pass" % name)
     if name == "rms":
         return torch.optim.RMSprop(params, lr=lr, weight_decay=weight_decay)
     if name == "sgd":
