@@ -290,6 +290,26 @@ int obman_adam_step(const obman_adam_tensor* tensors, int count, double lr, doub
                     double weight_decay, obman_stream_t stream);
 int obman_bf16_shadow(const float* src, uint16_t* dst, long n, obman_stream_t stream);
 
+/* ---- K17: softmax cross entropy against a table of classes ---------------------------------------
+ * loss[r] = log sum_v exp(x[r] . w[v] + b[v]) - (x[r] . w[t[r]] + b[t[r]]) without a [rows, classes] tensor of logits.
+ * x [rows, width], w [classes, width], bias [classes] (NULL = 0), row-major and contiguous, all of one type (0 fp32, 1 bf16,
+ * 2 fp16), at element alignment; target [rows] int64 (target_wide = 1) or int32.  Rows whose target is ignore_index count for
+ * nothing, whatever their x holds; another target outside [0, classes) makes the row's loss and every gradient NaN.
+ * reduction: 0 per row, 1 sum, 2 mean over the rows that are not ignored (0 if there are none).
+ * Forward: loss (rows floats, or one), lse [rows] and norm (one float: 1, or 1 / rows kept) are kept for the backward pass.
+ * Backward: g_loss (rows floats, or one); dx, dw, db of the inputs' type, each may be NULL.  The gradient of the logits exists for a
+ * piece of the classes at a time, in the scratch.  Fixed summation order: the same bits every call. */
+typedef struct obman_class_loss_params {
+  const void *x, *w, *bias, *target;
+  long rows, classes, ignore_index;
+  int width, type, target_wide, reduction;
+} obman_class_loss_params;
+long obman_class_loss_fwd_ws_bytes(const obman_class_loss_params* p);
+int obman_class_loss_fwd(const obman_class_loss_params* p, void* ws, float* loss, float* lse, float* norm, obman_stream_t stream);
+long obman_class_loss_bwd_ws_bytes(const obman_class_loss_params* p, int need_x, int need_w, int need_b);
+int obman_class_loss_bwd(const obman_class_loss_params* p, const float* lse, const float* norm, const float* g_loss, void* ws, void* dx,
+                         void* dw, void* db, obman_stream_t stream);
+
 /* ---- K16: the gradient norm over a list of tensors, clipping, and the clipped optimizer step -----
  * norm = (sum |g|^p)^(1/p) over all elements of all tensors (norm: 2 = L2, 1 = L1, 0 = largest |g|); clipping multiplies every
  * element by min(1, max_norm / (norm + 1e-6)) in fp32 and rounds once to the tensor's type (torch.nn.utils.clip_grad_norm_).

@@ -46,6 +46,10 @@ _SIGNATURES = {
     "obman_imgstream_ws_bytes": (_c_long, "iii"),
     "obman_imgstream_fwd": (_c_int, "piiip" "ii" "iii" "pp" "pp" "p"),
     "obman_adam_step": (_c_int, "pi" "ddddd" "p"),
+    "obman_class_loss_fwd_ws_bytes": (_c_long, "p"),
+    "obman_class_loss_fwd": (_c_int, "pp" "ppp" "p"),
+    "obman_class_loss_bwd_ws_bytes": (_c_long, "p" "iii"),
+    "obman_class_loss_bwd": (_c_int, "pppp" "p" "ppp" "p"),
     "obman_grad_norm_ws_doubles": (_c_long, "i"),
     "obman_grad_norm": (_c_int, "pppi" "i" "pp" "p"),
     "obman_grad_clip": (_c_int, "pppi" "if" "pp" "p"),
@@ -88,6 +92,11 @@ class PointGenGrads(ctypes.Structure):  # obman_pointgen_grads
 
 class AdamTensor(ctypes.Structure):  # obman_adam_tensor
     _fields_ = [("p", _fp), ("g", _fp), ("m", _fp), ("v", _fp), ("shadow_bf16", _fp), ("step", _fp), ("n", _c_long)]
+
+
+class ClassLossParams(ctypes.Structure):  # obman_class_loss_params
+    _fields_ = [("x", _fp), ("w", _fp), ("bias", _fp), ("target", _fp), ("rows", _c_long), ("classes", _c_long), ("ignore_index", _c_long),
+                ("width", _c_int), ("type", _c_int), ("target_wide", _c_int), ("reduction", _c_int)]
 
 
 class MseTerm(ctypes.Structure):  # obman_mse_term

@@ -914,3 +914,96 @@ def shadow_conv2d(conv, x):
     with torch.autocast("cuda", enabled=False):
         return _ShadowConv2d.apply(x.to(torch.bfloat16), w, sh, list(conv.stride), list(conv.padding), list(conv.dilation),
                                    conv.groups)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# Softmax cross entropy against a table of classes (csrc/classloss.hip)
+_CLASS_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
+def _class_loss_params(x, weight, bias, target, ignore_index, reduction):
+    p = _lib.ClassLossParams()
+    p.x, p.w, p.bias, p.target = x.data_ptr(), weight.data_ptr(), _ptr(bias), target.data_ptr()
+    p.rows, p.classes, p.ignore_index = target.numel(), weight.shape[0], ignore_index
+    p.width, p.type, p.target_wide, p.reduction = weight.shape[1], _CLASS_TYPES[weight.dtype], int(target.dtype == torch.int64), reduction
+    return p
+
+
+def _class_loss_ws(nbytes, what, device):
+    if nbytes < 0:
+        _lib.check(int(nbytes), what)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)  # of this call alone: recorded into a graph it is the graph's
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, target, ignore_index, reduction):
+        x, weight, target = x.contiguous(), weight.contiguous(), target.contiguous()
+        bias = None if bias is None else bias.contiguous()
+        rows, o = target.numel(), dict(dtype=torch.float32, device=x.device)
+        loss = torch.empty(target.shape if reduction == 0 else (), **o)
+        lse, norm = torch.empty(rows, **o), torch.empty((), **o)
+        lib = _lib.lib()
+        p = _class_loss_params(x, weight, bias, target, ignore_index, reduction)
+        with torch.cuda.device(x.device):
+            ws = _class_loss_ws(lib.obman_class_loss_fwd_ws_bytes(_ct.addressof(p)), "obman_class_loss_fwd_ws_bytes", x.device)
+            _lib.check(lib.obman_class_loss_fwd(_ct.addressof(p), ws.data_ptr(), loss.data_ptr(), lse.data_ptr(), norm.data_ptr(), _stream()),
+                       "obman_class_loss_fwd")
+        ctx.save_for_backward(x, weight, bias, target, lse, norm)
+        ctx.cfg = (ignore_index, reduction)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_loss):
+        x, weight, bias, target, lse, norm = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        g_loss = _dev(g_loss, "grad")
+        dx = torch.empty_like(x) if need_x else None
+        dw = torch.empty_like(weight) if need_w else None
+        db = torch.empty_like(bias) if need_b else None
+        lib = _lib.lib()
+        p = _class_loss_params(x, weight, bias, target, *ctx.cfg)
+        with torch.cuda.device(x.device):
+            ws = _class_loss_ws(lib.obman_class_loss_bwd_ws_bytes(_ct.addressof(p), int(need_x), int(need_w), int(need_b)),
+                                "obman_class_loss_bwd_ws_bytes", x.device)
+            _lib.check(lib.obman_class_loss_bwd(_ct.addressof(p), lse.data_ptr(), norm.data_ptr(), g_loss.data_ptr(), ws.data_ptr(), _ptr(dx),
+                                                _ptr(dw), _ptr(db), _stream()), "obman_class_loss_bwd")
+        return dx, dw, db, None, None, None
+
+
+def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduction="mean"):
+    """``F.cross_entropy(F.linear(x, weight, bias), target)`` without the logits: features ``x`` [..., width] classified against a table
+    ``weight`` [classes, width] - which vertex of a template a point belongs to, the nearest-vertex arg-mins of ``pairmin`` being such
+    targets.  Returns fp32 whatever the inputs' type: one value per row (``"none"``), their sum, or the mean over the rows kept.
+
+    ``x``, ``weight`` and ``bias`` [classes] are fp32, bf16 or fp16, all of one type (products of 16-bit types run on the matrix
+    cores as they are, fp32 ones as three fp16 products: 2^-22 relative); ``target`` [...] is int64 or int32.  A row whose target is
+    ``ignore_index`` has loss 0 and gradient 0 and takes no part in any gradient, even if its features are not finite; if every row
+    is ignored the mean is 0.  A target that is neither a class nor ``ignore_index`` makes the loss NaN.  A bias of -inf takes a class
+    out of the sum.  Gradients for ``x``, ``weight`` and ``bias`` (only those that need one are computed), once differentiable;
+    summation orders are fixed, so the same call gives the same bits."""
+    if reduction not in _REDUCTIONS:
+        raise ValueError("reduction must be 'none', 'sum' or 'mean', got %r" % (reduction,))
+    for name, t in (("x", x), ("weight", weight), ("target", target), ("bias", bias)):
+        if t is None and name == "bias":
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise _lib.ObmanHipError("%s must be a ROCm device tensor (the HIP path has no CPU fallback)" % name)
+        if t.device != x.device:
+            raise ValueError("x, weight, target and bias must be on one device, got %s and %s" % (x.device, t.device))
+    if x.dtype not in _CLASS_TYPES or weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
+        raise TypeError("x, weight and bias must all be fp32, bf16 or fp16, got %s, %s, %s" % (x.dtype, weight.dtype, None if bias is None else bias.dtype))
+    if target.dtype not in (torch.int64, torch.int32):
+        raise TypeError("target must be int64 or int32, got %s" % target.dtype)
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or target.shape != x.shape[:-1]:
+        raise ValueError("expected x [..., width], weight [classes, width], target [...]; got %s %s %s" % (tuple(x.shape), tuple(weight.shape), tuple(target.shape)))
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise ValueError("expected bias [classes], got %s for %d classes" % (tuple(bias.shape), weight.shape[0]))
+    if weight.shape[0] == 0 or not 0 < weight.shape[1] <= 16384:
+        raise ValueError("needs at least one class and a width of 1 .. 16384, got weight %s" % (tuple(weight.shape),))
+    if target.numel() == 0:  # no rows: nothing to launch; the graph stays connected
+        zero = x.float().sum() * 0.0
+        return x.float().sum(-1) if reduction == "none" else zero
+    return _LinearCrossEntropy.apply(x, weight, bias, target, int(ignore_index), _REDUCTIONS[reduction])
