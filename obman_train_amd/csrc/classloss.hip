@@ -50,6 +50,7 @@ struct Gemm {
   long k;                    // contraction, a multiple of 32
   long k_split;              // of it per block row of the grid's second axis
   int ti, tj;                // tiles
+  int k_tail;                // 0, or how many k rows of a are there in the last step (A_KR)
 };
 
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, unsigned lds, unsigned voff) {
@@ -60,13 +61,14 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, unsigned lds, un
 // One operand's tile: R rows (i or j) x 32 k.  KC: k contiguous in memory, LDS [row][64 bytes]; KR: a memory row is one k, LDS
 // [k][2 R bytes].  16-byte chunks are placed at (chunk ^ f(row)) so that neither the wide reads of KC (f = row >> 2 & 3) nor the
 // transposing reads of KR (f = 4 (k & 3)) meet in a bank; the DMA writes LDS linearly, so the source address carries the swizzle.
+// Every address is inside the operand: rows (KC) or columns (KR) behind the extent repeat the last ones and their results are not kept.
 template <bool KR, int R>
 struct Operand {
   static constexpr int N = R * BK * 2 / 1024 / 4;  // wave-wide loads per wave and step
-  const u16* base;
-  long plane, rows;
+  static constexpr int C = R / 8;                  // chunks of a k row (KR)
+  const u16* base;  // at the next step's k
+  long plane, rows, row0;
   int ld;
-  long row0;
   unsigned voff[N];
   __device__ __forceinline__ void init(const u16* p, long plane_, long rows_, int ld_, long row0_, int wave, int lane) {
     base = p; plane = plane_; rows = rows_; ld = ld_; row0 = row0_;
@@ -75,44 +77,43 @@ struct Operand {
       const int at = wave * N + q;
       if constexpr (!KR) {
         const int row = at * 16 + (lane >> 2), c = (lane & 3) ^ ((lane >> 4) & 3);
-        const long left = rows - 1 - row0;  // rows outside: the last one again, their results are not kept
+        const long left = rows - 1 - row0;
         voff[q] = (unsigned)((row < left ? row : left) * ld * 2 + c * 16);
       } else {
-        constexpr int C = R / 8;  // chunks of a k row
         const int k = at * (64 / C) + lane / C, c = (lane % C) ^ ((k & 3) << 2);
-        voff[q] = (unsigned)(k * ld * 2 + c * 16);
+        const int last = (int)(ld - row0) / 8 - 1;
+        voff[q] = (unsigned)(k * ld * 2 + (c < last ? c : last) * 16);
       }
     }
   }
-  __device__ __forceinline__ void issue(unsigned lds, int pl, long k, int wave, int lane) const {
-    const u16* p = base + (pl ? plane : 0);
-    long bytes;
-    if constexpr (!KR) { p += row0 * ld + k; bytes = ((rows - row0) * ld - k) * 2; }
-    else { p += k * ld + row0; bytes = ((rows - k) * ld - row0) * 2; }
-    if (bytes > 0x7ffffff0L) bytes = 0x7ffffff0L;
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<u16*>(p), 0, (int)bytes, 0x00020000);
-    const unsigned at = lds + wave * (N * 1024);
-    if (KR && k + BK > rows) {  // the table's last rows: repeat the last one, the other operand is zero there
-      constexpr int C = R / 8;
+  __device__ __forceinline__ const u16* at(const u16* p, int pl, long k) const {
+    return p + (pl ? plane : 0) + (KR ? k * ld + row0 : row0 * ld + k);
+  }
+  __device__ __forceinline__ void issue(unsigned lds, int wave, int lane, bool tail, int k_left) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<u16*>(base), 0, 0x7ffffff0, 0x00020000);
+    const unsigned to = lds + wave * (N * 1024);
+    if (KR && tail) {  // the table's last rows: the last one again, where the other operand is zero
 #pragma unroll
       for (int q = 0; q < N; ++q) {
-        const int kk = (wave * N + q) * (64 / C) + lane / C, last = (int)(rows - 1 - k);
-        dma16(r, at + q * 1024, voff[q] - (unsigned)((kk > last ? kk - last : 0) * ld * 2));
+        const int k = (wave * N + q) * (64 / C) + lane / C;
+        dma16(r, to + q * 1024, voff[q] - (unsigned)((k >= k_left ? k - k_left + 1 : 0) * ld * 2));
       }
     } else {
 #pragma unroll
-      for (int q = 0; q < N; ++q) dma16(r, at + q * 1024, voff[q]);
+      for (int q = 0; q < N; ++q) dma16(r, to + q * 1024, voff[q]);
     }
+    base += KR ? (long)BK * ld : BK;
   }
 };
 
 // fragment of 32 rows x 16 k: lane -> row lane % 32, k = 8 (lane / 32) .. + 7
 template <bool KR, int R>
 struct Frag {
-  unsigned off[KR ? 4 : 1];
+  unsigned off[KR ? 4 : 2];
   __device__ __forceinline__ void init(int first_row, int lane) {  // first_row: a multiple of 64 (of 128 where four fragments are read)
     if constexpr (!KR) {
-      off[0] = (first_row + (lane & 31)) * 64;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) off[ks] = (first_row + (lane & 31)) * 64 + ((2 * ks + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16;
     } else {
       const int k = 8 * (lane >> 5) + ((lane & 15) >> 2), kk = k & 3;
 #pragma unroll
@@ -124,8 +125,7 @@ struct Frag {
   }
   __device__ __forceinline__ u32x4 read(const char* tile, int f, int ks, int lane) const {
     if constexpr (!KR) {
-      const int c = (2 * ks + (lane >> 5)) ^ ((lane >> 2) & 3);
-      return *reinterpret_cast<const u32x4*>(tile + off[0] + f * 2048 + c * 16);
+      return *reinterpret_cast<const u32x4*>(tile + off[ks] + f * 2048);
     } else {
       const char* p = tile + off[f] + ks * 16 * (R * 2);
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p));
@@ -188,57 +188,113 @@ struct Ctx {
   char* smem;
 };
 
-// forward: per row (j) and tile of classes (i) the maximum and the sum of exponentials
-struct Stats {
+__device__ __forceinline__ void clear(f32x16 (&acc)[4][2]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+}
+
+// The bias of the tile's classes, -inf behind the last one, goes into LDS.  Without scales the accumulators start from it; a scaled
+// product adds it afterwards.
+template <bool SPLIT>
+struct Bias {
   Scale scale;
   const void* bias;
-  int bias_type;
+  int type;
+  long class0, classes;
+  __device__ __forceinline__ static const float* mine(const Ctx& c) {  // of this lane's classes: 8 q + 0 .. 3 from here on
+    return reinterpret_cast<const float*>(c.smem + STAGES * STAGE_BYTES) + c.wi * 128 + 4 * (c.lane >> 5);
+  }
+  __device__ __forceinline__ void before(const Ctx& c, f32x16 (&acc)[4][2]) const {
+    const long v0 = class0 + c.i0;
+    const bool plain = !bias && v0 + BI <= classes;
+    if (SPLIT || !plain) {
+      const long v = v0 + c.tid;
+      reinterpret_cast<float*>(c.smem + STAGES * STAGE_BYTES)[c.tid] = v >= classes ? -INFINITY : bias ? load_one(bias, type, v) : 0.f;
+    }
+    if (SPLIT || plain) {
+      clear(acc);
+      return;
+    }
+    __syncthreads();
+    const float* bl = mine(c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 b = *reinterpret_cast<const f32x4*>(bl + i * 32 + q * 8);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][q * 4 + e] = b[e];
+      }
+  }
+  // the logits in place of the sums; factor: what they come out multiplied by
+  __device__ __forceinline__ void finish(const Ctx& c, f32x16 (&acc)[4][2]) const {
+    if constexpr (SPLIT) {
+      const float s = scale.inverse();
+      const float* bl = mine(c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 b = *reinterpret_cast<const f32x4*>(bl + i * 32 + q * 8);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][q * 4 + e] = __builtin_fmaf(acc[i][j][q * 4 + e], s, b[e]);
+        }
+    }
+  }
+};
+
+// where a row's target is among this lane's 64 classes of a 128-wide half tile, or -1
+__device__ __forceinline__ int target_at(long target, long first_class, int lane) {
+  const long t = target - first_class - 4 * (lane >> 5);
+  return t >= 0 && t < 128 && !(t & 4) ? (int)t : -1;
+}
+
+// forward: per row (j) and tile of classes (i) the maximum and the sum of exponentials
+template <bool SPLIT>
+struct Stats {
+  Bias<SPLIT> bias;
   const void* target;
   int target_wide;
   float2* part;  // [ti][rows]
   float* picked; // [rows]
-  __device__ __forceinline__ void before(const Gemm& g, const Ctx& c) const {
-    float* bl = reinterpret_cast<float*>(c.smem + STAGES * STAGE_BYTES);
-    const long v = c.i0 + c.tid;
-    bl[c.tid] = v >= g.ni ? -INFINITY : bias ? load_one(bias, bias_type, v) : 0.f;
-  }
+  __device__ __forceinline__ void before(const Gemm&, const Ctx& c, f32x16 (&acc)[4][2]) const { bias.before(c, acc); }
   __device__ __forceinline__ void after(const Gemm& g, const Ctx& c, f32x16 (&acc)[4][2]) const {
-    const float s = scale.inverse();
-    const float* bl = reinterpret_cast<const float*>(c.smem + STAGES * STAGE_BYTES) + c.wi * 128 + 4 * (c.lane >> 5);
     float2* red = reinterpret_cast<float2*>(c.smem);
+    bias.finish(c, acc);
     float m[2], sum[2];
 #pragma unroll
     for (int fj = 0; fj < 2; ++fj) {
       const long r = c.j0 + c.wj * 64 + fj * 32 + (c.lane & 31);
-      long t = r < g.nj ? target_of(target, target_wide, r) - (c.i0 + c.wi * 128 + 4 * (c.lane >> 5)) : -1;
-      const int tt = t >= 0 && t < 128 ? (int)t : -1;
+      const int t = target_at(r < g.nj ? target_of(target, target_wide, r) : -1, c.i0 + c.wi * 128, c.lane);
+      if (__any(t >= 0)) {
+        float z = 0.f;
+#pragma unroll
+        for (int fi = 0; fi < 4; ++fi)
+#pragma unroll
+          for (int q = 0; q < 16; ++q) z = t == fi * 32 + (q >> 2) * 8 + (q & 3) ? acc[fi][fj][q] : z;
+        if (t >= 0) picked[r] = z;
+      }
       float top = -INFINITY;
 #pragma unroll
       for (int fi = 0; fi < 4; ++fi)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4 b = *reinterpret_cast<const f32x4*>(bl + fi * 32 + q * 8);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float z = acc[fi][fj][q * 4 + e] * s + b[e];
-            acc[fi][fj][q * 4 + e] = z;
-            top = fmaxf(top, z);
-          }
-        }
-      if (tt >= 0 && !(tt & 4)) {  // this lane's classes: 8 q' + 0 .. 3 from its first on
-#pragma unroll
-        for (int fi = 0; fi < 4; ++fi)
-#pragma unroll
-          for (int q = 0; q < 16; ++q)
-            if (tt == fi * 32 + (q >> 2) * 8 + (q & 3)) picked[r] = acc[fi][fj][q];
-      }
+        for (int q = 0; q < 16; q += 2) top = fmaxf(top, fmaxf(acc[fi][fj][q], acc[fi][fj][q + 1]));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       const float ref = top == -INFINITY ? 0.f : top * LOG2E;
-      float total = 0.f;
+      float part4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int fi = 0; fi < 4; ++fi)
 #pragma unroll
-        for (int q = 0; q < 16; ++q) total += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[fi][fj][q], LOG2E, -ref));
+        for (int q = 0; q < 16; ++q) part4[q & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[fi][fj][q], LOG2E, -ref));
+      float total = (part4[0] + part4[1]) + (part4[2] + part4[3]);
       total += __shfl_xor(total, 32, 64);
       m[fj] = top;
       sum[fj] = total;
@@ -259,59 +315,68 @@ struct Stats {
 };
 
 struct RowConst {  // per row of the backward pass
-  float lse2;      // lse in units of log 2
-  float c;         // weight of the row's gradient, scaled; 0 = ignored
-  int target;
-  int pad;
+  float lse2;      // (lse - log |c|) in units of log 2, +inf for a row without a gradient: g = exp2(z - lse2) is p |c| in one step
+  float c;         // |c|
+  int target;      // -1: none
+  unsigned sign;   // 0x80008000 where c < 0: the sign of two 16-bit values
 };
 
 // backward: g of a piece of the classes, [rows_padded][ld] in 16 bits
 template <int T, bool SPLIT>
 struct Grad {
-  Scale scale;
-  const void* bias;
-  int bias_type;
+  Bias<SPLIT> bias;
   const RowConst* rows;
-  long rows_padded, class0, classes;
+  long rows_padded;
   u16* out;
   long plane;
   int ld;
-  __device__ __forceinline__ void before(const Gemm&, const Ctx& c) const {
-    float* bl = reinterpret_cast<float*>(c.smem + STAGES * STAGE_BYTES);
-    const long v = class0 + c.i0 + c.tid;
-    bl[c.tid] = v >= classes ? -INFINITY : bias ? load_one(bias, bias_type, v) : 0.f;
-  }
+  __device__ __forceinline__ void before(const Gemm&, const Ctx& c, f32x16 (&acc)[4][2]) const { bias.before(c, acc); }
   __device__ __forceinline__ void after(const Gemm& g, const Ctx& c, f32x16 (&acc)[4][2]) const {
-    const float s = scale.inverse() * LOG2E;
-    const float* bl = reinterpret_cast<const float*>(c.smem + STAGES * STAGE_BYTES) + c.wi * 128 + 4 * (c.lane >> 5);
+    bias.finish(c, acc);
 #pragma unroll
     for (int fj = 0; fj < 2; ++fj) {
       const long r = c.j0 + c.wj * 64 + fj * 32 + (c.lane & 31);
-      if (r >= rows_padded) continue;
-      RowConst k = {0.f, 0.f, -1, 0};
+      RowConst k = {INFINITY, 0.f, -1, 0};
       if (r < g.nj) k = rows[r];
-      const long first = class0 + c.i0 + c.wi * 128 + 4 * (c.lane >> 5);
-      const long tl = (long)k.target - first;
-      const int t = tl >= 0 && tl < 128 ? (int)tl : -1;
-      u16* o = out + r * ld + (c.i0 + c.wi * 128 + 4 * (c.lane >> 5));
+      const int t = target_at(k.target, bias.class0 + c.i0 + c.wi * 128, c.lane);
 #pragma unroll
       for (int fi = 0; fi < 4; ++fi)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int at = fi * 32 + q * 8;
-          if (c.i0 + c.wi * 128 + at >= ld) continue;
-          const f32x4 b = *reinterpret_cast<const f32x4*>(bl + at);
-          u16 hi[4], lo[4];
+        for (int q = 0; q < 16; ++q) acc[fi][fj][q] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[fi][fj][q], LOG2E, -k.lse2));
+      if (__any(t >= 0)) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[fi][fj][q * 4 + e], s, __builtin_fmaf(b[e], LOG2E, -k.lse2)));
-            const float d = t == at + e ? p - 1.f : p;
-            const float x = k.c == 0.f ? 0.f : d * k.c;
-            hi[e] = narrow<T>(x);
-            if constexpr (SPLIT) lo[e] = narrow<T>(x - widen<T>(hi[e]));
+        for (int fi = 0; fi < 4; ++fi)
+#pragma unroll
+          for (int q = 0; q < 16; ++q) acc[fi][fj][q] -= t == fi * 32 + (q >> 2) * 8 + (q & 3) ? k.c : 0.f;
+      }
+      // lanes l and l + 32 hold classes 0 .. 3 and 4 .. 7 of each 8: an exchange gives each 8 in a row, 16 bytes
+      u16* o = out + r * ld + (c.i0 + c.wi * 128 + 8 * (c.lane >> 5));
+#pragma unroll
+      for (int fi = 0; fi < 4; ++fi)
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+          const int at = fi * 32 + q * 8;
+          unsigned hi[2][2], lo[2][2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float x = acc[fi][fj][(q + u) * 4 + e * 2], y = acc[fi][fj][(q + u) * 4 + e * 2 + 1];
+              const u16 hx = narrow<T>(x), hy = narrow<T>(y);
+              hi[u][e] = (hx | (unsigned)hy << 16) ^ k.sign;
+              if constexpr (SPLIT) lo[u][e] = (narrow<T>(x - widen<T>(hx)) | (unsigned)narrow<T>(y - widen<T>(hy)) << 16) ^ k.sign;
+            }
+          const bool keep = r < rows_padded && c.i0 + c.wi * 128 + at + 8 * (c.lane >> 5) < ld;
+          {
+            const u32x2 s0 = __builtin_amdgcn_permlane32_swap(hi[0][0], hi[1][0], false, false);
+            const u32x2 s1 = __builtin_amdgcn_permlane32_swap(hi[0][1], hi[1][1], false, false);
+            if (keep) *reinterpret_cast<u32x4*>(o + at) = u32x4{s0[0], s1[0], s0[1], s1[1]};
           }
-          *reinterpret_cast<u32x2*>(o + at) = u32x2{hi[0] | ((unsigned)hi[1] << 16), hi[2] | ((unsigned)hi[3] << 16)};
-          if constexpr (SPLIT) *reinterpret_cast<u32x2*>(o + plane + at) = u32x2{lo[0] | ((unsigned)lo[1] << 16), lo[2] | ((unsigned)lo[3] << 16)};
+          if constexpr (SPLIT) {
+            const u32x2 s0 = __builtin_amdgcn_permlane32_swap(lo[0][0], lo[1][0], false, false);
+            const u32x2 s1 = __builtin_amdgcn_permlane32_swap(lo[0][1], lo[1][1], false, false);
+            if (keep) *reinterpret_cast<u32x4*>(o + plane + at) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+          }
         }
     }
   }
@@ -322,7 +387,7 @@ struct Slab {
   float* out;
   long slab;
   int ld, add;
-  __device__ __forceinline__ void before(const Gemm&, const Ctx&) const {}
+  __device__ __forceinline__ void before(const Gemm&, const Ctx&, f32x16 (&acc)[4][2]) const { clear(acc); }
   __device__ __forceinline__ void after(const Gemm& g, const Ctx& c, f32x16 (&acc)[4][2]) const {
     float* o = out + c.split * slab;
 #pragma unroll
@@ -367,49 +432,54 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(Gemm g, Epi epi) {
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
 
   f32x16 acc[4][2];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-
-  long k_next = kb;
-  int term = TERMS == 3 ? 0 : 2, slot = 0;  // terms: lo hi, hi lo, hi hi
+  epi.before(g, ctx, acc);
+  int term = TERMS == 3 ? 0 : 2, left = (int)((ke - kb) / BK);  // terms: lo hi, hi lo, hi hi
+  const int per_term = left;
+  oa.base = oa.at(g.a, term == 0, kb);
+  ob.base = ob.at(g.b, term == 1, kb);
+  const bool tail = g.k_tail && ke == g.k;  // the last step runs over the end of the table
+  unsigned to = lds0;
   const auto issue = [&]() {
-    const unsigned at = lds0 + slot * STAGE_BYTES;
-    oa.issue(at, term == 0, k_next, wave, lane);
-    ob.issue(at + A_BYTES, term == 1, k_next, wave, lane);
-    slot = slot == STAGES - 1 ? 0 : slot + 1;
-    k_next += BK;
-    if (k_next >= ke) { k_next = kb; ++term; }
+    oa.issue(to, wave, lane, A_KR && tail && left == 1, g.k_tail);
+    ob.issue(to + A_BYTES, wave, lane, false, 0);
+    to = to == lds0 + (STAGES - 1) * STAGE_BYTES ? lds0 : to + STAGE_BYTES;
+    --left;
+    if (TERMS == 3 && left == 0) {
+      left = per_term;
+      ++term;
+      oa.base = oa.at(g.a, 0, kb);
+      ob.base = ob.at(g.b, term == 1, kb);
+    }
   };
   constexpr int PER = Operand<A_KR, BI>::N + Operand<B_KR, BJ>::N;
   static_assert(PER == 6, "the counted wait below");
-  epi.before(g, ctx);
   if (steps > 0) issue();
   if (steps > 1) issue();
-  int cur = 0;
+  const char* from = smem;
   for (int s = 0; s < steps; ++s) {
     // step s has arrived for every wave (only step s + 1 may still be under way), and every wave has read step s - 1, whose slot is next
     if (s + 1 < steps) asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (s + 2 < steps) issue();
-    const char* ta = smem + cur * STAGE_BYTES;
-    const char* tb = ta + A_BYTES;
-    cur = cur == STAGES - 1 ? 0 : cur + 1;
+    u32x4 a[2][4], b[2][2];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      u32x4 a[4], b[2];
 #pragma unroll
-      for (int f = 0; f < 2; ++f) b[f] = fb.read(tb, f, ks, lane);
+      for (int f = 0; f < 2; ++f) b[ks][f] = fb.read(from + A_BYTES, f, ks, lane);
 #pragma unroll
-      for (int f = 0; f < 4; ++f) a[f] = fa.read(ta, f, ks, lane);
+      for (int f = 0; f < 4; ++f) a[ks][f] = fa.read(from, f, ks, lane);
+    }
+    if (s + 2 < steps) issue();
+    from = from == smem + (STAGES - 1) * STAGE_BYTES ? smem : from + STAGE_BYTES;
+    __builtin_amdgcn_sched_barrier(0);  // all reads go out before the first product waits for one
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
       for (int f = 0; f < 4; ++f)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) acc[f][h] = mfma<T>(a[f], b[h], acc[f][h]);
-    }
+        for (int h = 0; h < 2; ++h) acc[f][h] = mfma<T>(a[ks][f], b[ks][h], acc[f][h]);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
   }
   __syncthreads();
   epi.after(g, ctx, acc);
@@ -589,10 +659,11 @@ __global__ __launch_bounds__(1024) void rows_kernel(const float* __restrict__ ls
   if (r >= rows) return;
   const long t = target_of(target, wide, r);
   RowConst k;
-  k.lse2 = lse[r] * LOG2E;
-  k.c = t == ignore ? 0.f : (per_row ? g_loss[r] * down : 1.f) * g_scale;
-  k.target = t == ignore || t < 0 || t > 0x7fffffffL ? -1 : (int)t;
-  k.pad = 0;
+  const float w = t == ignore ? 0.f : (per_row ? g_loss[r] * down : 1.f) * g_scale;
+  k.c = fabsf(w);
+  k.lse2 = w == 0.f ? INFINITY : lse[r] * LOG2E - log2f(k.c);
+  k.target = w == 0.f || t < 0 || t > 0x7fffffffL ? -1 : (int)t;
+  k.sign = w < 0.f ? 0x80008000u : 0u;
   out[r] = k;
 }
 
@@ -660,12 +731,18 @@ static bool in_place(const obman_class_loss_params& p, const void* q) {
   return p.type != F32 && p.width % BK == 0 && ((size_t)q & 15) == 0;
 }
 
-// how many parts the contraction is cut into: tiles * n fills whole rounds of the slots, the result fits few slabs
+// Into how many parts the contraction is cut: the fewest step times of 32 over all rounds of the slots, a part costing START steps
+// more (its pipeline's start and its slab)
+constexpr long START = 40;
 static int split_of(long tiles, long k) {
-  if (tiles >= SLOTS) return 1;
-  long n = SLOTS / tiles, most = k / 256 < 1 ? 1 : k / 256;
-  n = n < most ? n : most;
-  return (int)(n > 64 ? 64 : n < 1 ? 1 : n);
+  long best = 0;
+  int n = 1;
+  for (int c = 1; c <= 64; ++c) {
+    if (c > 1 && k / c < 256) break;
+    const long t = (tiles * c + SLOTS - 1) / SLOTS * (k / BK / c + START);
+    if (c == 1 || t < best) { best = t; n = c; }
+  }
+  return n;
 }
 static long split_len(long k, int n) { return up((k + n - 1) / n, BK); }
 
@@ -766,15 +843,15 @@ static int check(const obman_class_loss_params* p) {
 
 template <int T, int TERMS>
 static int forward(const obman_class_loss_params& p, const Work& o, hipStream_t st) {
-  const bool split = TERMS == 3;
-  const Gemm g{o.w.p, o.x.p, o.w.plane, o.x.plane, p.classes, p.rows, o.w.ld, o.x.ld, p.classes, p.rows, o.w.ld, o.w.ld, o.ti, obman_cdiv(p.rows, BJ)};
-  const Stats epi{Scale{split ? o.scales : nullptr, split ? o.scales + 1 : nullptr}, p.bias, p.type, p.target, p.target_wide, o.part, o.picked};
-  return launch_gemm<false, false, Stats, T, TERMS>(g, 1, epi, st);
+  constexpr bool split = TERMS == 3;
+  const Gemm g{o.w.p, o.x.p, o.w.plane, o.x.plane, p.classes, p.rows, o.w.ld, o.x.ld, p.classes, p.rows, o.w.ld, o.w.ld, o.ti, obman_cdiv(p.rows, BJ), 0};
+  const Stats<split> epi{{Scale{split ? o.scales : nullptr, split ? o.scales + 1 : nullptr}, p.bias, p.type, 0, p.classes}, p.target, p.target_wide, o.part, o.picked};
+  return launch_gemm<false, false, Stats<split>, T, TERMS>(g, 1, epi, st);
 }
 
 template <int T, int TERMS>
 static int backward(const obman_class_loss_params& p, const Work& o, void* dx, void* dw, void* db, hipStream_t st) {
-  const bool split = TERMS == 3;
+  constexpr bool split = TERMS == 3;
   const float *sx = split ? o.scales : nullptr, *sw = split ? o.scales + 1 : nullptr;
   const long xr = o.x.rows;
   const int ld = o.w.ld, size = p.type == F32 ? 4 : 2;
@@ -782,16 +859,16 @@ static int backward(const obman_class_loss_params& p, const Work& o, void* dx, v
   for (long v0 = 0; v0 < p.classes; v0 += o.piece) {
     const long nv = p.classes - v0 < o.piece ? p.classes - v0 : o.piece, kv = up(nv, BK);
     const u16* wp = o.w.p + v0 * ld;
-    const Gemm gg{wp, o.x.p, o.w.plane, o.x.plane, p.classes - v0, xr, ld, ld, kv, p.rows, ld, ld, obman_cdiv(kv, BI), obman_cdiv(xr, BJ)};
-    const Grad<T, TERMS == 3> ge{Scale{sx, sw}, p.bias, p.type, o.rows, xr, v0, v0 + nv, o.g, o.g_plane, (int)kv};
-    if ((e = launch_gemm<false, false, Grad<T, TERMS == 3>, T, TERMS>(gg, 1, ge, st))) return e;
+    const Gemm gg{wp, o.x.p, o.w.plane, o.x.plane, p.classes - v0, xr, ld, ld, kv, p.rows, ld, ld, obman_cdiv(kv, BI), obman_cdiv(xr, BJ), 0};
+    const Grad<T, split> ge{{Scale{sx, sw}, p.bias, p.type, v0, v0 + nv}, o.rows, xr, o.g, o.g_plane, (int)kv};
+    if ((e = launch_gemm<false, false, Grad<T, split>, T, TERMS>(gg, 1, ge, st))) return e;
     if (dx) {
-      const Gemm gx{wp, o.g, o.w.plane, o.g_plane, p.classes - v0, xr, ld, (int)kv, ld, p.rows, kv, split_len(kv, o.dx_split), obman_cdiv(ld, BI), obman_cdiv(p.rows, BJ)};
+      const Gemm gx{wp, o.g, o.w.plane, o.g_plane, p.classes - v0, xr, ld, (int)kv, ld, p.rows, kv, split_len(kv, o.dx_split), obman_cdiv(ld, BI), obman_cdiv(p.rows, BJ), nv == kv ? 0 : (int)(nv - (kv - BK))};
       const Slab ex{o.dx_slabs, p.rows * ld, ld, v0 > 0};
       if ((e = launch_gemm<true, false, Slab, T, TERMS>(gx, o.dx_split, ex, st))) return e;
     }
     if (dw || db) {
-      const Gemm gw{o.x.p, o.g, o.x.plane, o.g_plane, xr, xr, ld, (int)kv, ld, nv, xr, split_len(xr, o.dw_split), obman_cdiv(ld, BI), obman_cdiv(nv, BJ)};
+      const Gemm gw{o.x.p, o.g, o.x.plane, o.g_plane, xr, xr, ld, (int)kv, ld, nv, xr, split_len(xr, o.dw_split), obman_cdiv(ld, BI), obman_cdiv(nv, BJ), 0};
       const Slab ew{o.dw_slabs, o.piece * ld, ld, 0};
       if ((e = launch_gemm<true, true, Slab, T, TERMS>(gw, o.dw_split, ew, st))) return e;
       finish_kernel<<<blocks_for(nv * (ld / 4)), 256, 0, st>>>(o.dw_slabs, o.dw_split, o.piece * ld, nv, ld, p.width, o.alpha, Scale{sx, nullptr},
