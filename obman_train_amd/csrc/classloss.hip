@@ -30,27 +30,34 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 typedef u16 u16x8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef u16 u16x4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 enum { F32 = 0, BF16 = 1, F16 = 2 };
 
+// Operands are kept in blocks of 32 columns, [columns / 32][rows][32]: whatever a step of 32 needs of one - 32 columns of 256 rows, or
+// 32 rows of 8 blocks - is read in runs of 1 KB or more.  (Row-major, a step reads 64 of each row's bytes, half cache lines: the path
+// from L2 to LDS then holds the products at 900 Tflop/s; without any such reads they run at 1170 - 1270.)  Rows are padded with zeros
+// to whole tiles, so no address leaves an operand.
 constexpr int BI = 256, BJ = 128, BK = 32;  // tile: 256 x 128, four waves of 128 x 64; 72 KB of LDS, so two blocks share a CU and one's
 constexpr int STAGES = 3;                    // epilogue runs beside the other's products
+constexpr long MOST_ROWS = 1L << 22;         // of an operand: eight blocks of its columns stay within 32-bit offsets
 constexpr int A_BYTES = BI * BK * 2, B_BYTES = BJ * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr int LDS_BYTES = STAGES * STAGE_BYTES + BI * 4;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float G_SCALE = 16384.f;  // |g| / max|c| <= 1 in fp16
 
+struct Side {       // [planes][blocks][rows][32]
+  const u16* p;
+  long plane, rows; // elements from the hi to the lo plane; rows of a block
+};
 struct Gemm {
-  const u16 *a, *b;          // [planes][rows][ld]
-  long a_plane, b_plane;     // elements from the hi to the lo plane
-  long a_rows, b_rows;       // rows of memory (a contiguous-k operand: its i or j extent; else: its k extent)
-  int lda, ldb;
-  long ni, nj;               // extents of the result
-  long k;                    // contraction, a multiple of 32
-  long k_split;              // of it per block row of the grid's second axis
-  int ti, tj;                // tiles
-  int k_tail;                // 0, or how many k rows of a are there in the last step (A_KR)
+  Side a, b;
+  long ni, nj;      // extents of the result
+  long k;           // contraction, a multiple of 32
+  long k_split;     // of it per block row of the grid's second axis
+  int ti, tj;       // tiles
+  int na, nb;       // column blocks of a / b (an operand whose rows are contracted: tiles that run over its columns repeat the last block)
 };
 
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, unsigned lds, unsigned voff) {
@@ -58,80 +65,57 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, unsigned lds, un
   asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(r) : "memory", "m0");
 }
 
-// One operand's tile: R rows (i or j) x 32 k.  KC: k contiguous in memory, LDS [row][64 bytes]; KR: a memory row is one k, LDS
-// [k][2 R bytes].  16-byte chunks are placed at (chunk ^ f(row)) so that neither the wide reads of KC (f = row >> 2 & 3) nor the
-// transposing reads of KR (f = 4 (k & 3)) meet in a bank; the DMA writes LDS linearly, so the source address carries the swizzle.
-// Every address is inside the operand: rows (KC) or columns (KR) behind the extent repeat the last ones and their results are not kept.
+// One operand's tile, R (i or j) x 32 k, 64-byte rows in LDS.  KC: the rows are i or j and the 32 columns are k; 16-byte chunks are placed at
+// chunk ^ (row >> 2 & 3), so that the wide reads do not meet in a bank (the DMA writes LDS linearly: the source address carries the
+// swizzle).  KR: the rows are k, 32 of them for each of R / 32 column blocks, read by the transposing LDS reads, which take four
+// whole rows at a time and need no swizzle.
 template <bool KR, int R>
 struct Operand {
-  static constexpr int N = R * BK * 2 / 1024 / 4;  // wave-wide loads per wave and step
-  static constexpr int C = R / 8;                  // chunks of a k row (KR)
+  static constexpr int N = R * BK * 2 / 1024 / 4;  // wave-wide loads of 1 KB per wave and step
   const u16* base;  // at the next step's k
-  long plane, rows, row0;
-  int ld;
+  long step;
   unsigned voff[N];
-  __device__ __forceinline__ void init(const u16* p, long plane_, long rows_, int ld_, long row0_, int wave, int lane) {
-    base = p; plane = plane_; rows = rows_; ld = ld_; row0 = row0_;
+  __device__ __forceinline__ void init(const Side& s, int first_block, int blocks, int wave, int lane) {
+    step = KR ? BK * 32 : s.rows * 32;
 #pragma unroll
     for (int q = 0; q < N; ++q) {
       const int at = wave * N + q;
       if constexpr (!KR) {
-        const int row = at * 16 + (lane >> 2), c = (lane & 3) ^ ((lane >> 4) & 3);
-        const long left = rows - 1 - row0;
-        voff[q] = (unsigned)((row < left ? row : left) * ld * 2 + c * 16);
+        voff[q] = at * 1024 + (lane >> 2) * 64 + ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
       } else {
-        const int k = at * (64 / C) + lane / C, c = (lane % C) ^ ((k & 3) << 2);
-        const int last = (int)(ld - row0) / 8 - 1;
-        voff[q] = (unsigned)(k * ld * 2 + (c < last ? c : last) * 16);
+        const int last = blocks - 1 - first_block, b = at >> 1;
+        voff[q] = (unsigned)((b < last ? b : last) * s.rows * 64 + (at & 1) * 1024 + lane * 16);
       }
     }
   }
-  __device__ __forceinline__ const u16* at(const u16* p, int pl, long k) const {
-    return p + (pl ? plane : 0) + (KR ? k * ld + row0 : row0 * ld + k);
-  }
-  __device__ __forceinline__ void issue(unsigned lds, int wave, int lane, bool tail, int k_left) {
+  // row0: first row (KC: of the tile; KR: of the contraction), k0: first column of the contraction (KC) or of the tile (KR)
+  __device__ __forceinline__ void start(const Side& s, int pl, long row0, long col0) { base = s.p + (pl ? s.plane : 0) + (col0 * s.rows + row0 * 32); }
+  __device__ __forceinline__ void issue(unsigned lds, int wave) {
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<u16*>(base), 0, 0x7ffffff0, 0x00020000);
-    const unsigned to = lds + wave * (N * 1024);
-    if (KR && tail) {  // the table's last rows: the last one again, where the other operand is zero
 #pragma unroll
-      for (int q = 0; q < N; ++q) {
-        const int k = (wave * N + q) * (64 / C) + lane / C;
-        dma16(r, to + q * 1024, voff[q] - (unsigned)((k >= k_left ? k - k_left + 1 : 0) * ld * 2));
-      }
-    } else {
-#pragma unroll
-      for (int q = 0; q < N; ++q) dma16(r, to + q * 1024, voff[q]);
-    }
-    base += KR ? (long)BK * ld : BK;
+    for (int q = 0; q < N; ++q) dma16(r, lds + wave * (N * 1024) + q * 1024, voff[q]);
+    base += step;
   }
 };
 
 // fragment of 32 rows x 16 k: lane -> row lane % 32, k = 8 (lane / 32) .. + 7
-template <bool KR, int R>
+template <bool KR>
 struct Frag {
-  unsigned off[KR ? 4 : 2];
-  __device__ __forceinline__ void init(int first_row, int lane) {  // first_row: a multiple of 64 (of 128 where four fragments are read)
-    if constexpr (!KR) {
+  unsigned off[2];
+  __device__ __forceinline__ void init(int first_row, int lane) {  // first_row: a multiple of 32
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) off[ks] = (first_row + (lane & 31)) * 64 + ((2 * ks + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16;
-    } else {
-      const int k = 8 * (lane >> 5) + ((lane & 15) >> 2), kk = k & 3;
-#pragma unroll
-      for (int f = 0; f < 4; ++f) {
-        const int chunk = ((first_row / 8 + f * 4) ^ (kk << 2)) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-        off[f] = k * (R * 2) + chunk * 16 + (lane & 1) * 8;
-      }
+    for (int ks = 0; ks < 2; ++ks) {
+      if constexpr (!KR) off[ks] = (first_row + (lane & 31)) * 64 + ((2 * ks + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16;
+      // the transposing read: in a group of 16 lanes, lane c receives element c of the four rows that lanes 4 r .. 4 r + 3 point at
+      else off[ks] = first_row * 64 + (ks * 16 + 8 * (lane >> 5) + ((lane & 15) >> 2)) * 64 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
     }
   }
-  __device__ __forceinline__ u32x4 read(const char* tile, int f, int ks, int lane) const {
-    if constexpr (!KR) {
-      return *reinterpret_cast<const u32x4*>(tile + off[ks] + f * 2048);
-    } else {
-      const char* p = tile + off[f] + ks * 16 * (R * 2);
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p + 4 * (R * 2)));
-      return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-    }
+  __device__ __forceinline__ u32x4 read(const char* tile, int f, int ks) const {
+    const char* p = tile + off[ks] + f * 2048;
+    if constexpr (!KR) return *reinterpret_cast<const u32x4*>(p);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p + 4 * 64));
+    return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 };
 
@@ -184,7 +168,7 @@ struct Scale {
 
 struct Ctx {
   long i0, j0;
-  int wi, wj, lane, wave, tid, ti_index, split;
+  int wi, wj, lane, tid, ti_index, tj_index, split;
   char* smem;
 };
 
@@ -316,12 +300,12 @@ struct Stats {
 
 struct RowConst {  // per row of the backward pass
   float lse2;      // (lse - log |c|) in units of log 2, +inf for a row without a gradient: g = exp2(z - lse2) is p |c| in one step
-  float c;         // |c|
+  float c;
   int target;      // -1: none
-  unsigned sign;   // 0x80008000 where c < 0: the sign of two 16-bit values
+  int pad;
 };
 
-// backward: g of a piece of the classes, [rows_padded][ld] in 16 bits
+// backward: g of a piece of the classes, blocks of 32 classes like every operand; its column sums over the tile's rows on request
 template <int T, bool SPLIT>
 struct Grad {
   Bias<SPLIT> bias;
@@ -329,7 +313,8 @@ struct Grad {
   long rows_padded;
   u16* out;
   long plane;
-  int ld;
+  int columns;      // of out
+  float* sums;      // [tj][columns]: the bias gradient's parts, summed before g is rounded
   __device__ __forceinline__ void before(const Gemm&, const Ctx& c, f32x16 (&acc)[4][2]) const { bias.before(c, acc); }
   __device__ __forceinline__ void after(const Gemm& g, const Ctx& c, f32x16 (&acc)[4][2]) const {
     bias.finish(c, acc);
@@ -347,15 +332,22 @@ struct Grad {
 #pragma unroll
         for (int fi = 0; fi < 4; ++fi)
 #pragma unroll
-          for (int q = 0; q < 16; ++q) acc[fi][fj][q] -= t == fi * 32 + (q >> 2) * 8 + (q & 3) ? k.c : 0.f;
+          for (int q = 0; q < 16; ++q) acc[fi][fj][q] -= t == fi * 32 + (q >> 2) * 8 + (q & 3) ? fabsf(k.c) : 0.f;
+      }
+      if (__any(k.c < 0.f)) {
+        const float sign = k.c < 0.f ? -1.f : 1.f;
+#pragma unroll
+        for (int fi = 0; fi < 4; ++fi)
+#pragma unroll
+          for (int q = 0; q < 16; ++q) acc[fi][fj][q] *= sign;
       }
       // lanes l and l + 32 hold classes 0 .. 3 and 4 .. 7 of each 8: an exchange gives each 8 in a row, 16 bytes
-      u16* o = out + r * ld + (c.i0 + c.wi * 128 + 8 * (c.lane >> 5));
+      u16* o = out + ((c.i0 + c.wi * 128) * rows_padded + r * 32) + 8 * (c.lane >> 5);
 #pragma unroll
-      for (int fi = 0; fi < 4; ++fi)
+      for (int fi = 0; fi < 4; ++fi) {
+        if (c.i0 + c.wi * 128 + fi * 32 >= columns) continue;
 #pragma unroll
         for (int q = 0; q < 4; q += 2) {
-          const int at = fi * 32 + q * 8;
           unsigned hi[2][2], lo[2][2];
 #pragma unroll
           for (int u = 0; u < 2; ++u)
@@ -363,22 +355,43 @@ struct Grad {
             for (int e = 0; e < 2; ++e) {
               const float x = acc[fi][fj][(q + u) * 4 + e * 2], y = acc[fi][fj][(q + u) * 4 + e * 2 + 1];
               const u16 hx = narrow<T>(x), hy = narrow<T>(y);
-              hi[u][e] = (hx | (unsigned)hy << 16) ^ k.sign;
-              if constexpr (SPLIT) lo[u][e] = (narrow<T>(x - widen<T>(hx)) | (unsigned)narrow<T>(y - widen<T>(hy)) << 16) ^ k.sign;
+              hi[u][e] = hx | (unsigned)hy << 16;
+              if constexpr (SPLIT) lo[u][e] = narrow<T>(x - widen<T>(hx)) | (unsigned)narrow<T>(y - widen<T>(hy)) << 16;
             }
-          const bool keep = r < rows_padded && c.i0 + c.wi * 128 + at + 8 * (c.lane >> 5) < ld;
+          u16* to = o + fi * 32 * rows_padded + q * 8;
           {
             const u32x2 s0 = __builtin_amdgcn_permlane32_swap(hi[0][0], hi[1][0], false, false);
             const u32x2 s1 = __builtin_amdgcn_permlane32_swap(hi[0][1], hi[1][1], false, false);
-            if (keep) *reinterpret_cast<u32x4*>(o + at) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+            *reinterpret_cast<u32x4*>(to) = u32x4{s0[0], s1[0], s0[1], s1[1]};
           }
           if constexpr (SPLIT) {
             const u32x2 s0 = __builtin_amdgcn_permlane32_swap(lo[0][0], lo[1][0], false, false);
             const u32x2 s1 = __builtin_amdgcn_permlane32_swap(lo[0][1], lo[1][1], false, false);
-            if (keep) *reinterpret_cast<u32x4*>(o + plane + at) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+            *reinterpret_cast<u32x4*>(to + plane) = u32x4{s0[0], s1[0], s0[1], s1[1]};
           }
         }
+      }
     }
+    if (!sums) return;
+    // over the 16 lanes of a row of lanes in registers, then [wj][half][class] in LDS
+    float* red = reinterpret_cast<float*>(c.smem);
+    const int l16 = c.lane & 15;
+#pragma unroll
+    for (int fi = 0; fi < 4; ++fi) {
+      float mine = 0.f;
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        float v = acc[fi][0][q] + acc[fi][1][q];
+        v += obman_dpp<0xB1>(v);
+        v += obman_dpp<0x4E>(v);
+        v += obman_dpp<0x141>(v);
+        v += obman_dpp<0x140>(v);
+        mine = l16 == q ? v : mine;
+      }
+      red[(c.wj * 2 + ((c.lane >> 4) & 1)) * 256 + c.wi * 128 + fi * 32 + (l16 >> 2) * 8 + 4 * (c.lane >> 5) + (l16 & 3)] = mine;
+    }
+    __syncthreads();
+    if (c.i0 + c.tid < columns) sums[(long)c.tj_index * columns + c.i0 + c.tid] = (red[c.tid] + red[256 + c.tid]) + (red[512 + c.tid] + red[768 + c.tid]);
   }
 };
 
@@ -418,13 +431,13 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(Gemm g, Epi epi) {
   tile_of(g, bi, bj);
   bi = __builtin_amdgcn_readfirstlane(bi);
   bj = __builtin_amdgcn_readfirstlane(bj);
-  const Ctx ctx{(long)bi * BI, (long)bj * BJ, wave & 1, wave >> 1, lane, wave, tid, bi, (int)blockIdx.y, smem};
+  const Ctx ctx{(long)bi * BI, (long)bj * BJ, wave & 1, wave >> 1, lane, tid, bi, bj, (int)blockIdx.y, smem};
   Operand<A_KR, BI> oa;
   Operand<B_KR, BJ> ob;
-  oa.init(g.a, g.a_plane, g.a_rows, g.lda, ctx.i0, wave, lane);
-  ob.init(g.b, g.b_plane, g.b_rows, g.ldb, ctx.j0, wave, lane);
-  Frag<A_KR, BI> fa;
-  Frag<B_KR, BJ> fb;
+  oa.init(g.a, bi * (BI / 32), g.na, wave, lane);
+  ob.init(g.b, bj * (BJ / 32), g.nb, wave, lane);
+  Frag<A_KR> fa;
+  Frag<B_KR> fb;
   fa.init(ctx.wi * 128, lane);
   fb.init(ctx.wj * 64, lane);
   const long kb = (long)blockIdx.y * g.k_split, ke = kb + g.k_split < g.k ? kb + g.k_split : g.k;
@@ -435,20 +448,20 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(Gemm g, Epi epi) {
   epi.before(g, ctx, acc);
   int term = TERMS == 3 ? 0 : 2, left = (int)((ke - kb) / BK);  // terms: lo hi, hi lo, hi hi
   const int per_term = left;
-  oa.base = oa.at(g.a, term == 0, kb);
-  ob.base = ob.at(g.b, term == 1, kb);
-  const bool tail = g.k_tail && ke == g.k;  // the last step runs over the end of the table
+  const auto start = [&]() {
+    oa.start(g.a, term == 0, A_KR ? kb : ctx.i0, A_KR ? ctx.i0 : kb);
+    ob.start(g.b, term == 1, B_KR ? kb : ctx.j0, B_KR ? ctx.j0 : kb);
+  };
+  start();
   unsigned to = lds0;
   const auto issue = [&]() {
-    oa.issue(to, wave, lane, A_KR && tail && left == 1, g.k_tail);
-    ob.issue(to + A_BYTES, wave, lane, false, 0);
+    oa.issue(to, wave);
+    ob.issue(to + A_BYTES, wave);
     to = to == lds0 + (STAGES - 1) * STAGE_BYTES ? lds0 : to + STAGE_BYTES;
-    --left;
-    if (TERMS == 3 && left == 0) {
+    if (TERMS == 3 && --left == 0) {
       left = per_term;
       ++term;
-      oa.base = oa.at(g.a, 0, kb);
-      ob.base = ob.at(g.b, term == 1, kb);
+      start();
     }
   };
   constexpr int PER = Operand<A_KR, BI>::N + Operand<B_KR, BJ>::N;
@@ -464,9 +477,9 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(Gemm g, Epi epi) {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
-      for (int f = 0; f < 2; ++f) b[ks][f] = fb.read(from + A_BYTES, f, ks, lane);
+      for (int f = 0; f < 2; ++f) b[ks][f] = fb.read(from + A_BYTES, f, ks);
 #pragma unroll
-      for (int f = 0; f < 4; ++f) a[ks][f] = fa.read(from, f, ks, lane);
+      for (int f = 0; f < 4; ++f) a[ks][f] = fa.read(from, f, ks);
     }
     if (s + 2 < steps) issue();
     from = from == smem + (STAGES - 1) * STAGE_BYTES ? smem : from + STAGE_BYTES;
@@ -487,87 +500,101 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(Gemm g, Epi epi) {
 
 // ------------------------------------------------------------------------------------------------------- operands and rows
 
-// largest finite |x| of the kept rows: 256 block maxima
-__global__ __launch_bounds__(256) void absmax_kernel(const float* __restrict__ x, long rows, int width, const void* target, int wide, long ignore, float* __restrict__ part) {
+// largest finite |x| of the kept rows of x (grid row 0) and of w (1): MAX_PARTS block maxima each
+constexpr int MAX_PARTS = 512;
+__global__ __launch_bounds__(256) void absmax_kernel(const float* __restrict__ x, long rows, const float* __restrict__ w, long classes, int width, const void* target, int wide,
+                                                    long ignore, float* __restrict__ part) {
+  const bool first = blockIdx.y == 0;
+  const float* p = first ? x : w;
+  const long n = first ? rows : classes;
+  const int lane = threadIdx.x & 63, full = width & ~3;
   float m = 0.f;
-  const long n = rows * width;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += 256L * 256) {
-    const float a = fabsf(x[i]);
-    if (a > m && a < INFINITY && (!target || target_of(target, wide, i / width) != ignore)) m = a;
+  for (long r = (long)blockIdx.x * 4 + (threadIdx.x >> 6); r < n; r += MAX_PARTS * 4) {  // a wave takes a row
+    if (first && target_of(target, wide, r) == ignore) continue;
+    const float* q = p + r * width;
+    for (int i = lane * 4; i < full; i += 256) {
+      const f32x4u v = *reinterpret_cast<const f32x4u*>(q + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { const float a = fabsf(v[e]); m = a > m && a < INFINITY ? a : m; }
+    }
+    if (full + lane < width) { const float a = fabsf(q[full + lane]); m = a > m && a < INFINITY ? a : m; }
   }
   m = obman_wave_max(m);
   __shared__ float red[4];
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  if (lane == 0) red[threadIdx.x >> 6] = m;
   __syncthreads();
-  if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  if (threadIdx.x == 0) part[blockIdx.y * MAX_PARTS + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
-// the power of two that brings the largest element to 2^13 .. 2^14 (1 for an all-zero tensor)
-__global__ __launch_bounds__(256) void scale_kernel(const float* __restrict__ part, float* __restrict__ scale) {
-  float m = obman_wave_max(part[(size_t)blockIdx.x * 256 + threadIdx.x]);
+// the power of two that brings the largest element to 2^13 .. 2^14 (1 for an all-zero tensor); every thread of the block has it
+__device__ float scale_of(const float* __restrict__ part) {
   __shared__ float red[4];
+  float m = fmaxf(part[threadIdx.x], part[threadIdx.x + 256]);
+  m = obman_wave_max(m);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    int e = 0;
-    if (m > 0.f) (void)frexpf(m, &e);  // m = f 2^e, f in [0.5, 1)
-    e = 14 - e;
-    e = e > 126 ? 126 : e < -126 ? -126 : e;
-    scale[blockIdx.x] = m > 0.f ? ldexpf(1.f, e) : 1.f;
-  }
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  int e = 0;
+  if (m > 0.f) (void)frexpf(m, &e);  // m = f 2^e, f in [0.5, 1)
+  e = 14 - e;
+  e = e > 60 ? 60 : e < -60 ? -60 : e;  // two of them multiply within fp32
+  return m > 0.f ? ldexpf(1.f, e) : 1.f;
 }
 
-// rows of an operand into 16-bit planes [planes][rows_padded][ld]: zeros behind the width, for ignored rows and behind the last row;
-// `ones`: column `width` is 1 (its product with g is the gradient of the bias)
+// x (grid row 0) and w (1) into blocks of 32 columns, [planes][blocks][padded rows][32]: zeros behind the width, behind the last row
+// and for ignored rows
+struct Pack { const void* src; u16* dst; long rows, padded, plane; };
 template <int TYPE>
-__global__ __launch_bounds__(256) void pack_kernel(const void* __restrict__ src, long rows, long rows_padded, int width, int ld, const void* target, int wide, long ignore,
-                                                  int ones, const float* __restrict__ scale, u16* __restrict__ dst, long plane) {
-  const int per = ld >> 3;
-  const long n = rows_padded * per;
-  const float sc = TYPE == F32 ? *scale : 1.f;
+__global__ __launch_bounds__(256) void pack_kernel(Pack px, Pack pw, int width, int chunks, const void* target, int wide, long ignore, const float* __restrict__ part,
+                                                  float* __restrict__ scale) {
+  const bool first = blockIdx.y == 0;
+  const Pack p = first ? px : pw;
+  float sc = 1.f;
+  if constexpr (TYPE == F32) {
+    sc = scale_of(part + blockIdx.y * MAX_PARTS);
+    if (blockIdx.x == 0 && threadIdx.x == 0) scale[blockIdx.y] = sc;
+  }
+  const long n = p.padded * chunks;  // of 8 columns
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
-    const long r = i / per;
-    const int c = (int)(i - r * per) * 8;
-    const bool keep = r < rows && (!target || target_of(target, wide, r) != ignore);
+    const long r = i / chunks;
+    const int c = (int)(i - r * chunks) * 8;
     u16 hi[8], lo[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) hi[e] = lo[e] = 0;
-    if (keep) {
+    if (r < p.rows && (!first || target_of(target, wide, r) != ignore)) {
       const long at = r * width + c;
       if constexpr (TYPE == F32) {
-        const float* p = static_cast<const float*>(src) + at;
+        const float* q = static_cast<const float*>(p.src) + at;
         float v[8];
         if (c + 8 <= width) {
-          const f32x4u a = *reinterpret_cast<const f32x4u*>(p), b = *reinterpret_cast<const f32x4u*>(p + 4);
+          const f32x4u a = *reinterpret_cast<const f32x4u*>(q), b = *reinterpret_cast<const f32x4u*>(q + 4);
 #pragma unroll
           for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[e + 4] = b[e]; }
         } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = c + e < width ? p[e] : 0.f;
+          for (int e = 0; e < 8; ++e) v[e] = c + e < width ? q[e] : 0.f;
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float y = v[e] * sc;
           hi[e] = narrow<F16>(y);
-          const float rest = y - widen<F16>(hi[e]);
-          lo[e] = fabsf(y) < INFINITY ? narrow<F16>(rest) : (u16)0;
+          lo[e] = fabsf(y) < INFINITY ? narrow<F16>(y - widen<F16>(hi[e])) : (u16)0;
         }
       } else {
-        const u16* p = static_cast<const u16*>(src) + at;
+        const u16* q = static_cast<const u16*>(p.src) + at;
         if (c + 8 <= width) {
-          const u16x8u a = *reinterpret_cast<const u16x8u*>(p);
+          const u16x8u a = *reinterpret_cast<const u16x8u*>(q);
 #pragma unroll
           for (int e = 0; e < 8; ++e) hi[e] = a[e];
         } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) hi[e] = c + e < width ? p[e] : (u16)0;
+          for (int e = 0; e < 8; ++e) hi[e] = c + e < width ? q[e] : (u16)0;
         }
       }
-      if (ones && width >= c && width < c + 8) hi[width - c] = TYPE == F32 ? narrow<F16>(1.f) : TYPE == BF16 ? narrow<BF16>(1.f) : narrow<F16>(1.f);
     }
-    *reinterpret_cast<u32x4*>(dst + r * ld + c) = *reinterpret_cast<u32x4*>(hi);
-    if constexpr (TYPE == F32) *reinterpret_cast<u32x4*>(dst + plane + r * ld + c) = *reinterpret_cast<u32x4*>(lo);
+    u16* o = p.dst + ((long)(c >> 5) * p.padded + r) * 32 + (c & 31);
+    *reinterpret_cast<u32x4*>(o) = *reinterpret_cast<u32x4*>(hi);
+    if constexpr (TYPE == F32) *reinterpret_cast<u32x4*>(o + p.plane) = *reinterpret_cast<u32x4*>(lo);
   }
 }
 
@@ -660,32 +687,49 @@ __global__ __launch_bounds__(1024) void rows_kernel(const float* __restrict__ ls
   const long t = target_of(target, wide, r);
   RowConst k;
   const float w = t == ignore ? 0.f : (per_row ? g_loss[r] * down : 1.f) * g_scale;
-  k.c = fabsf(w);
-  k.lse2 = w == 0.f ? INFINITY : lse[r] * LOG2E - log2f(k.c);
+  k.c = w;
+  k.lse2 = w == 0.f ? INFINITY : lse[r] * LOG2E - log2f(fabsf(w));
   k.target = w == 0.f || t < 0 || t > 0x7fffffffL ? -1 : (int)t;
-  k.sign = w < 0.f ? 0x80008000u : 0u;
+  k.pad = 0;
   out[r] = k;
 }
 
-// sum of the slabs times alpha into the gradient's own type; column `width` is the bias gradient
-__global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ slabs, int n, long slab, long rows, int ld, int width, const float* __restrict__ alpha, Scale scale,
-                                                    void* __restrict__ out, int type, void* __restrict__ bias_out) {
-  const float k = *alpha * scale.inverse();
-  const int per = ld >> 2;
+// sum of the slabs times alpha into the gradient's own type
+__global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ slabs, int n, long slab, long rows, int ld, int width, const float* __restrict__ alpha,
+                                                    const float* __restrict__ scale, void* __restrict__ out, int type) {
+  const float k = *alpha * (scale ? 1.f / *scale : 1.f);
+  const int per = (width + 3) >> 2;
   const long total = rows * per;
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
     const long r = i / per;
     const int c = (int)(i - r * per) * 4;
-    if (c > width || (c == width && !bias_out)) continue;
     const float* p = slabs + r * ld + c;
     f32x4 v = *reinterpret_cast<const f32x4*>(p);
     for (int s = 1; s < n; ++s) v += *reinterpret_cast<const f32x4*>(p + s * slab);
+    const long at = r * width + c;
+    if (c + 4 <= width) {
+      if (type == F32) *reinterpret_cast<f32x4u*>(static_cast<float*>(out) + at) = f32x4u{v[0] * k, v[1] * k, v[2] * k, v[3] * k};
+      else {
+        u16x4u o;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (c + e < width) { if (out) store_one(out, type, r * width + c + e, v[e] * k); }
-      else if (c + e == width && bias_out) store_one(bias_out, type, r, v[e] * (*alpha));
+        for (int e = 0; e < 4; ++e) o[e] = type == BF16 ? narrow<BF16>(v[e] * k) : narrow<F16>(v[e] * k);
+        *reinterpret_cast<u16x4u*>(static_cast<u16*>(out) + at) = o;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < width) store_one(out, type, at + e, v[e] * k);
     }
   }
+}
+
+// the bias gradient: the column sums of the tiles of rows, in order
+__global__ __launch_bounds__(256) void bias_kernel(const float* __restrict__ sums, int n, int columns, long classes, const float* __restrict__ alpha, void* __restrict__ out, int type) {
+  const long v = (long)blockIdx.x * 256 + threadIdx.x;
+  if (v >= classes) return;
+  double s = 0.0;
+  for (int t = 0; t < n; ++t) s += sums[(long)t * columns + v];
+  store_one(out, type, v, (float)(s * *alpha));
 }
 
 // --------------------------------------------------------------------------------------------------------------- the calls
@@ -706,29 +750,49 @@ struct Carve {  // scratch: offsets first, pointers once a base is there
 constexpr long PIECE_BYTES = 512L << 20;  // of g at a time
 constexpr int SLOTS = 512;                // blocks that run at a time: two per CU
 
-struct Packed { u16* p; long plane; int ld; long rows; };
+// what the forward pass leaves for the backward pass: both operands in blocks, and their scales
+struct Keep {
+  Side x, w;
+  u16 *xp, *wp;
+  float* scales;
+  int blocks;  // of 32 columns
+  size_t bytes;
+};
+static Keep keep_of(const obman_class_loss_params& p, void* mem) {
+  Carve c{static_cast<char*>(mem)};
+  Keep k;
+  const int planes = p.type == F32 ? 2 : 1;
+  const long xr = up(p.rows, BJ), wr = up(p.classes, BI);
+  k.blocks = obman_cdiv(p.width, 32);
+  const long xn = xr * k.blocks * 32, wn = wr * k.blocks * 32;
+  k.scales = c.take<float>(2);
+  k.xp = c.take<u16>(xn * planes);
+  k.wp = c.take<u16>(wn * planes);
+  k.x = {k.xp, xn, xr};
+  k.w = {k.wp, wn, wr};
+  k.bytes = c.at;
+  return k;
+}
 
-struct Work {
-  // both directions
-  float *max_part, *scales;
-  Packed x, w;
-  // forward
+struct Forward {
+  float* max_part;
   float2* part;
   float* picked;
   double2* sums;
   int ti, row_blocks;
-  // backward
-  RowConst* rows;
-  float* alpha;
-  u16* g;
-  long g_plane, piece;
-  float *dx_slabs, *dw_slabs;
-  int dx_split, dw_split;
   size_t bytes;
 };
-
-static bool in_place(const obman_class_loss_params& p, const void* q) {
-  return p.type != F32 && p.width % BK == 0 && ((size_t)q & 15) == 0;
+static Forward forward_of(const obman_class_loss_params& p, void* mem) {
+  Carve c{static_cast<char*>(mem)};
+  Forward o;
+  o.ti = obman_cdiv(p.classes, BI);
+  o.row_blocks = obman_cdiv(p.rows, 64);
+  o.max_part = c.take<float>(2 * MAX_PARTS);
+  o.part = c.take<float2>((size_t)o.ti * p.rows);
+  o.picked = c.take<float>(p.rows);
+  o.sums = c.take<double2>(o.row_blocks);
+  o.bytes = c.at;
+  return o;
 }
 
 // Into how many parts the contraction is cut: the fewest step times of 32 over all rounds of the slots, a part costing START steps
@@ -746,44 +810,34 @@ static int split_of(long tiles, long k) {
 }
 static long split_len(long k, int n) { return up((k + n - 1) / n, BK); }
 
-static Work plan(const obman_class_loss_params& p, void* ws, bool back, bool need_x, bool need_w, bool need_b) {
-  Work o;
-  Carve c{static_cast<char*>(ws)};
-  const bool split = p.type == F32;
-  const int planes = split ? 2 : 1;
-  o.max_part = c.take<float>(split ? 512 : 0);
-  o.scales = c.take<float>(4);
-  const bool bias_col = back && need_b;
-  const int ld = (int)up(p.width + (bias_col ? 1 : 0), BK);
-  const bool wrap = !in_place(p, p.w) || ld != p.width, xpack = back || !in_place(p, p.x);
-  const long xr = back ? up(p.rows, BK) : p.rows;
-  o.x = {xpack ? c.take<u16>((size_t)planes * xr * ld) : nullptr, xr * ld, ld, xr};
-  o.w = {wrap ? c.take<u16>((size_t)planes * p.classes * ld) : nullptr, p.classes * ld, ld, p.classes};
-  if (!xpack) o.x = {static_cast<u16*>(const_cast<void*>(p.x)), 0, p.width, p.rows};
-  if (!wrap) o.w = {static_cast<u16*>(const_cast<void*>(p.w)), 0, p.width, p.classes};
-  if (!back) {
-    o.ti = obman_cdiv(p.classes, BI);
-    o.row_blocks = obman_cdiv(p.rows, 64);
-    o.part = c.take<float2>((size_t)o.ti * p.rows);
-    o.picked = c.take<float>(p.rows);
-    o.sums = c.take<double2>(o.row_blocks);
-  } else {
-    o.rows = c.take<RowConst>(p.rows);
-    o.alpha = c.take<float>(1);
-    long piece = PIECE_BYTES / (xr * 2 * planes) / BI * BI;
-    if (piece < 2 * BI) piece = 2 * BI;
-    const long all = up(p.classes, BK);
-    if (piece >= all) piece = all;
-    else piece = up(up(p.classes, BK) / ((p.classes + piece - 1) / piece) + BI, BI);  // equal pieces
-    o.piece = piece > all ? all : piece;
-    o.g_plane = xr * o.piece;
-    o.g = c.take<u16>((size_t)planes * xr * o.piece);
-    const long dx_tiles = (long)obman_cdiv(ld, BI) * obman_cdiv(p.rows, BJ), dw_tiles = (long)obman_cdiv(ld, BI) * obman_cdiv(o.piece, BJ);
-    o.dx_split = split_of(dx_tiles, o.piece);
-    o.dw_split = split_of(dw_tiles, xr);
-    o.dx_slabs = c.take<float>(need_x ? (size_t)o.dx_split * p.rows * ld : 0);
-    o.dw_slabs = c.take<float>(need_w || need_b ? (size_t)o.dw_split * o.piece * ld : 0);
-  }
+struct Backward {
+  RowConst* rows;
+  float* alpha;
+  u16* g;
+  long g_plane, piece;
+  float *dx_slabs, *dw_slabs, *sums;
+  int dx_split, dw_split;
+  size_t bytes;
+};
+static Backward backward_of(const obman_class_loss_params& p, const Keep& k, void* mem, bool need_x, bool need_w, bool need_b) {
+  Carve c{static_cast<char*>(mem)};
+  Backward o;
+  const int planes = p.type == F32 ? 2 : 1, ld = k.blocks * 32;
+  const long xr = k.x.rows, all = up(p.classes, 32);
+  o.rows = c.take<RowConst>(p.rows);
+  o.alpha = c.take<float>(1);
+  long most = PIECE_BYTES / (xr * 2 * planes) / BI * BI;
+  if (most < 2 * BI) most = 2 * BI;
+  o.piece = all;
+  if (most < all) o.piece = up(all / ((all + most - 1) / most) + 1, BI);  // equal pieces
+  if (o.piece > all) o.piece = all;
+  o.g_plane = xr * o.piece;
+  o.g = c.take<u16>((size_t)planes * xr * o.piece);
+  o.dx_split = split_of((long)obman_cdiv(ld, BI) * obman_cdiv(p.rows, BJ), o.piece);
+  o.dw_split = split_of((long)obman_cdiv(ld, BI) * obman_cdiv(o.piece, BJ), xr);
+  o.dx_slabs = c.take<float>(need_x ? (size_t)o.dx_split * p.rows * ld : 0);
+  o.dw_slabs = c.take<float>(need_w ? (size_t)o.dw_split * o.piece * ld : 0);
+  o.sums = c.take<float>(need_b ? (size_t)(xr / BJ) * o.piece : 0);
   o.bytes = c.at;
   return o;
 }
@@ -807,78 +861,72 @@ static int launch_gemm(const Gemm& g, int splits, const Epi& epi, hipStream_t st
   return 0;
 }
 
-static int pack(const obman_class_loss_params& p, const void* src, long rows, const Packed& d, bool masked, bool ones, const float* scale, hipStream_t st) {
-  const void* t = masked ? p.target : nullptr;
-  const int blocks = blocks_for(d.rows * (d.ld / 8));
-  if (p.type == F32) pack_kernel<F32><<<blocks, 256, 0, st>>>(src, rows, d.rows, p.width, d.ld, t, p.target_wide, p.ignore_index, ones, scale, d.p, d.plane);
-  else if (p.type == BF16) pack_kernel<BF16><<<blocks, 256, 0, st>>>(src, rows, d.rows, p.width, d.ld, t, p.target_wide, p.ignore_index, ones, scale, d.p, d.plane);
-  else pack_kernel<F16><<<blocks, 256, 0, st>>>(src, rows, d.rows, p.width, d.ld, t, p.target_wide, p.ignore_index, ones, scale, d.p, d.plane);
-  OBMAN_LAUNCH_CHECK();
-  return 0;
-}
-
-static int operands(const obman_class_loss_params& p, const Work& o, bool ones, hipStream_t st) {
+static int operands(const obman_class_loss_params& p, const Keep& k, float* max_part, hipStream_t st) {
   if (p.type == F32) {
-    absmax_kernel<<<256, 256, 0, st>>>(static_cast<const float*>(p.x), p.rows, p.width, p.target, p.target_wide, p.ignore_index, o.max_part);
-    OBMAN_LAUNCH_CHECK();
-    absmax_kernel<<<256, 256, 0, st>>>(static_cast<const float*>(p.w), p.classes, p.width, nullptr, 0, 0, o.max_part + 256);
-    OBMAN_LAUNCH_CHECK();
-    scale_kernel<<<2, 256, 0, st>>>(o.max_part, o.scales);
+    absmax_kernel<<<dim3(MAX_PARTS, 2), 256, 0, st>>>(static_cast<const float*>(p.x), p.rows, static_cast<const float*>(p.w), p.classes, p.width, p.target, p.target_wide,
+                                                      p.ignore_index, max_part);
     OBMAN_LAUNCH_CHECK();
   }
-  int e = 0;
-  if (o.x.p != p.x) e = pack(p, p.x, p.rows, o.x, true, ones, o.scales, st);
-  if (!e && o.w.p != p.w) e = pack(p, p.w, p.classes, o.w, false, false, o.scales + 1, st);
-  return e;
+  const Pack px{p.x, k.xp, p.rows, k.x.rows, k.x.plane}, pw{p.w, k.wp, p.classes, k.w.rows, k.w.plane};
+  const long rows = px.padded > pw.padded ? px.padded : pw.padded;
+  const dim3 grid(blocks_for(rows * k.blocks * 4), 2);
+  if (p.type == F32) pack_kernel<F32><<<grid, 256, 0, st>>>(px, pw, p.width, k.blocks * 4, p.target, p.target_wide, p.ignore_index, max_part, k.scales);
+  else if (p.type == BF16) pack_kernel<BF16><<<grid, 256, 0, st>>>(px, pw, p.width, k.blocks * 4, p.target, p.target_wide, p.ignore_index, max_part, k.scales);
+  else pack_kernel<F16><<<grid, 256, 0, st>>>(px, pw, p.width, k.blocks * 4, p.target, p.target_wide, p.ignore_index, max_part, k.scales);
+  OBMAN_LAUNCH_CHECK();
+  return 0;
 }
 
 static int check(const obman_class_loss_params* p) {
   if (!p || !p->x || !p->w || !p->target) return -1;
   if (p->rows <= 0 || p->classes <= 0 || p->width <= 0 || p->width > 16384) return -2;
-  if (p->rows > 0x7fffffffL || p->classes > 0x7fffff00L) return -2;
+  if (p->rows > MOST_ROWS || p->classes > MOST_ROWS) return -2;
   if (p->type < 0 || p->type > 2 || p->reduction < 0 || p->reduction > 2) return -3;
-  if ((long)obman_cdiv(p->classes, BI) * obman_cdiv(p->rows, BJ) > 0x7fffffffL) return -4;
   return 0;
 }
 
 template <int T, int TERMS>
-static int forward(const obman_class_loss_params& p, const Work& o, hipStream_t st) {
+static int forward(const obman_class_loss_params& p, const Keep& k, const Forward& o, hipStream_t st) {
   constexpr bool split = TERMS == 3;
-  const Gemm g{o.w.p, o.x.p, o.w.plane, o.x.plane, p.classes, p.rows, o.w.ld, o.x.ld, p.classes, p.rows, o.w.ld, o.w.ld, o.ti, obman_cdiv(p.rows, BJ), 0};
-  const Stats<split> epi{{Scale{split ? o.scales : nullptr, split ? o.scales + 1 : nullptr}, p.bias, p.type, 0, p.classes}, p.target, p.target_wide, o.part, o.picked};
+  const long kk = k.blocks * 32;
+  const Gemm g{k.w, k.x, p.classes, p.rows, kk, kk, o.ti, obman_cdiv(p.rows, BJ), 0, 0};
+  const Stats<split> epi{{Scale{split ? k.scales : nullptr, split ? k.scales + 1 : nullptr}, p.bias, p.type, 0, p.classes}, p.target, p.target_wide, o.part, o.picked};
   return launch_gemm<false, false, Stats<split>, T, TERMS>(g, 1, epi, st);
 }
 
 template <int T, int TERMS>
-static int backward(const obman_class_loss_params& p, const Work& o, void* dx, void* dw, void* db, hipStream_t st) {
+static int backward(const obman_class_loss_params& p, const Keep& k, const Backward& o, void* dx, void* dw, void* db, hipStream_t st) {
   constexpr bool split = TERMS == 3;
-  const float *sx = split ? o.scales : nullptr, *sw = split ? o.scales + 1 : nullptr;
-  const long xr = o.x.rows;
-  const int ld = o.w.ld, size = p.type == F32 ? 4 : 2;
+  const float *sx = split ? k.scales : nullptr, *sw = split ? k.scales + 1 : nullptr;
+  const long xr = k.x.rows;
+  const int ld = k.blocks * 32, size = p.type == F32 ? 4 : 2;
   int e;
   for (long v0 = 0; v0 < p.classes; v0 += o.piece) {
-    const long nv = p.classes - v0 < o.piece ? p.classes - v0 : o.piece, kv = up(nv, BK);
-    const u16* wp = o.w.p + v0 * ld;
-    const Gemm gg{wp, o.x.p, o.w.plane, o.x.plane, p.classes - v0, xr, ld, ld, kv, p.rows, ld, ld, obman_cdiv(kv, BI), obman_cdiv(xr, BJ), 0};
-    const Grad<T, split> ge{{Scale{sx, sw}, p.bias, p.type, v0, v0 + nv}, o.rows, xr, o.g, o.g_plane, (int)kv};
+    const long nv = p.classes - v0 < o.piece ? p.classes - v0 : o.piece, kv = up(nv, 32);
+    const Side w{k.wp + v0 * 32, k.w.plane, k.w.rows}, gs{o.g, o.g_plane, xr};
+    const Gemm gg{w, k.x, kv, p.rows, ld, ld, obman_cdiv(kv, BI), (int)(xr / BJ), 0, 0};
+    const Grad<T, split> ge{{Scale{sx, sw}, p.bias, p.type, v0, v0 + nv}, o.rows, xr, o.g, o.g_plane, (int)kv, db ? o.sums : nullptr};
     if ((e = launch_gemm<false, false, Grad<T, split>, T, TERMS>(gg, 1, ge, st))) return e;
     if (dx) {
-      const Gemm gx{wp, o.g, o.w.plane, o.g_plane, p.classes - v0, xr, ld, (int)kv, ld, p.rows, kv, split_len(kv, o.dx_split), obman_cdiv(ld, BI), obman_cdiv(p.rows, BJ), nv == kv ? 0 : (int)(nv - (kv - BK))};
+      const Gemm gx{w, gs, ld, p.rows, kv, split_len(kv, o.dx_split), obman_cdiv(ld, BI), obman_cdiv(p.rows, BJ), k.blocks, 0};
       const Slab ex{o.dx_slabs, p.rows * ld, ld, v0 > 0};
       if ((e = launch_gemm<true, false, Slab, T, TERMS>(gx, o.dx_split, ex, st))) return e;
     }
-    if (dw || db) {
-      const Gemm gw{o.x.p, o.g, o.x.plane, o.g_plane, xr, xr, ld, (int)kv, ld, nv, xr, split_len(xr, o.dw_split), obman_cdiv(ld, BI), obman_cdiv(nv, BJ), 0};
+    if (dw) {
+      const Gemm gw{k.x, gs, ld, nv, xr, split_len(xr, o.dw_split), obman_cdiv(ld, BI), obman_cdiv(nv, BJ), k.blocks, (int)(kv / 32)};
       const Slab ew{o.dw_slabs, o.piece * ld, ld, 0};
       if ((e = launch_gemm<true, true, Slab, T, TERMS>(gw, o.dw_split, ew, st))) return e;
-      finish_kernel<<<blocks_for(nv * (ld / 4)), 256, 0, st>>>(o.dw_slabs, o.dw_split, o.piece * ld, nv, ld, p.width, o.alpha, Scale{sx, nullptr},
-                                                               dw ? static_cast<char*>(dw) + (size_t)v0 * p.width * size : nullptr, p.type,
-                                                               db ? static_cast<char*>(db) + (size_t)v0 * size : nullptr);
+      finish_kernel<<<blocks_for(nv * (p.width / 4 + 1)), 256, 0, st>>>(o.dw_slabs, o.dw_split, o.piece * ld, nv, ld, p.width, o.alpha, sx,
+                                                                        static_cast<char*>(dw) + (size_t)v0 * p.width * size, p.type);
+      OBMAN_LAUNCH_CHECK();
+    }
+    if (db) {
+      bias_kernel<<<obman_cdiv(nv, 256), 256, 0, st>>>(o.sums, (int)(xr / BJ), (int)kv, nv, o.alpha, static_cast<char*>(db) + (size_t)v0 * size, p.type);
       OBMAN_LAUNCH_CHECK();
     }
   }
   if (dx) {
-    finish_kernel<<<blocks_for(p.rows * (ld / 4)), 256, 0, st>>>(o.dx_slabs, o.dx_split, p.rows * ld, p.rows, ld, p.width, o.alpha, Scale{sw, nullptr}, dx, p.type, nullptr);
+    finish_kernel<<<blocks_for(p.rows * (p.width / 4 + 1)), 256, 0, st>>>(o.dx_slabs, o.dx_split, p.rows * ld, p.rows, ld, p.width, o.alpha, sw, dx, p.type);
     OBMAN_LAUNCH_CHECK();
   }
   return 0;
@@ -888,19 +936,27 @@ static int backward(const obman_class_loss_params& p, const Work& o, void* dx, v
 
 extern "C" {
 
-long obman_class_loss_fwd_ws_bytes(const obman_class_loss_params* p) {
+long obman_class_loss_keep_bytes(const obman_class_loss_params* p) {
   const int e = cl::check(p);
-  return e ? e : (long)cl::plan(*p, nullptr, false, false, false, false).bytes;
+  return e ? e : (long)cl::keep_of(*p, nullptr).bytes;
 }
 
-int obman_class_loss_fwd(const obman_class_loss_params* p, void* ws, float* loss, float* lse, float* norm, obman_stream_t stream) {
+long obman_class_loss_fwd_ws_bytes(const obman_class_loss_params* p) {
+  const int e = cl::check(p);
+  return e ? e : (long)cl::forward_of(*p, nullptr).bytes;
+}
+
+int obman_class_loss_fwd(const obman_class_loss_params* p, void* keep, void* ws, float* loss, float* lse, float* norm, obman_stream_t stream) {
   int e = cl::check(p);
   if (e) return e;
-  if (!ws || !loss || !lse || !norm) return -1;
+  if (!keep || !ws || !loss || !lse || !norm) return -1;
   hipStream_t st = (hipStream_t)stream;
-  const cl::Work o = cl::plan(*p, ws, false, false, false, false);
-  if ((e = cl::operands(*p, o, false, st))) return e;
-  e = p->type == cl::F32 ? cl::forward<cl::F16, 3>(*p, o, st) : p->type == cl::BF16 ? cl::forward<cl::BF16, 1>(*p, o, st) : cl::forward<cl::F16, 1>(*p, o, st);
+  const cl::Keep k = cl::keep_of(*p, keep);
+  const cl::Forward o = cl::forward_of(*p, ws);
+  if ((e = cl::operands(*p, k, o.max_part, st))) return e;
+  e = p->type == cl::F32    ? cl::forward<cl::F16, 3>(*p, k, o, st)
+      : p->type == cl::BF16 ? cl::forward<cl::BF16, 1>(*p, k, o, st)
+                            : cl::forward<cl::F16, 1>(*p, k, o, st);
   if (e) return e;
   cl::join_rows_kernel<<<o.row_blocks, 256, 0, st>>>(o.part, o.ti, p->rows, p->classes, o.picked, p->target, p->target_wide, p->ignore_index, lse,
                                                      p->reduction ? nullptr : loss, p->reduction ? o.sums : nullptr);
@@ -914,24 +970,24 @@ int obman_class_loss_fwd(const obman_class_loss_params* p, void* ws, float* loss
 
 long obman_class_loss_bwd_ws_bytes(const obman_class_loss_params* p, int need_x, int need_w, int need_b) {
   const int e = cl::check(p);
-  return e ? e : (long)cl::plan(*p, nullptr, true, need_x, need_w, need_b).bytes;
+  return e ? e : (long)cl::backward_of(*p, cl::keep_of(*p, nullptr), nullptr, need_x, need_w, need_b).bytes;
 }
 
-int obman_class_loss_bwd(const obman_class_loss_params* p, const float* lse, const float* norm, const float* g_loss, void* ws, void* dx, void* dw, void* db,
-                         obman_stream_t stream) {
+int obman_class_loss_bwd(const obman_class_loss_params* p, const void* keep, const float* lse, const float* norm, const float* g_loss, void* ws, void* dx, void* dw,
+                         void* db, obman_stream_t stream) {
   int e = cl::check(p);
   if (e) return e;
-  if (!ws || !lse || !g_loss || (p->reduction && !norm)) return -1;
+  if (!keep || !ws || !lse || !g_loss || (p->reduction && !norm)) return -1;
   if (!dx && !dw && !db) return 0;
   hipStream_t st = (hipStream_t)stream;
-  const cl::Work o = cl::plan(*p, ws, true, dx != nullptr, dw != nullptr, db != nullptr);
-  if ((e = cl::operands(*p, o, db != nullptr, st))) return e;
+  const cl::Keep k = cl::keep_of(*p, const_cast<void*>(keep));
+  const cl::Backward o = cl::backward_of(*p, k, ws, dx != nullptr, dw != nullptr, db != nullptr);
   cl::rows_kernel<<<obman_cdiv(p->rows, 1024), 1024, 0, st>>>(lse, p->target, p->target_wide, p->ignore_index, p->rows, g_loss, p->reduction == 0, norm,
                                                               p->type == cl::BF16 ? 1.f : cl::G_SCALE, o.rows, o.alpha);
   OBMAN_LAUNCH_CHECK();
-  return p->type == cl::F32    ? cl::backward<cl::F16, 3>(*p, o, dx, dw, db, st)
-         : p->type == cl::BF16 ? cl::backward<cl::BF16, 1>(*p, o, dx, dw, db, st)
-                               : cl::backward<cl::F16, 1>(*p, o, dx, dw, db, st);
+  return p->type == cl::F32    ? cl::backward<cl::F16, 3>(*p, k, o, dx, dw, db, st)
+         : p->type == cl::BF16 ? cl::backward<cl::BF16, 1>(*p, k, o, dx, dw, db, st)
+                               : cl::backward<cl::F16, 1>(*p, k, o, dx, dw, db, st);
 }
 
 }  // extern "C"

@@ -947,17 +947,18 @@ class _LinearCrossEntropy(torch.autograd.Function):
         lib = _lib.lib()
         p = _class_loss_params(x, weight, bias, target, ignore_index, reduction)
         with torch.cuda.device(x.device):
+            keep = _class_loss_ws(lib.obman_class_loss_keep_bytes(_ct.addressof(p)), "obman_class_loss_keep_bytes", x.device)
             ws = _class_loss_ws(lib.obman_class_loss_fwd_ws_bytes(_ct.addressof(p)), "obman_class_loss_fwd_ws_bytes", x.device)
-            _lib.check(lib.obman_class_loss_fwd(_ct.addressof(p), ws.data_ptr(), loss.data_ptr(), lse.data_ptr(), norm.data_ptr(), _stream()),
+            _lib.check(lib.obman_class_loss_fwd(_ct.addressof(p), keep.data_ptr(), ws.data_ptr(), loss.data_ptr(), lse.data_ptr(), norm.data_ptr(), _stream()),
                        "obman_class_loss_fwd")
-        ctx.save_for_backward(x, weight, bias, target, lse, norm)
+        ctx.save_for_backward(x, weight, bias, target, keep, lse, norm)
         ctx.cfg = (ignore_index, reduction)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss):
-        x, weight, bias, target, lse, norm = ctx.saved_tensors
+        x, weight, bias, target, keep, lse, norm = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         g_loss = _dev(g_loss, "grad")
         dx = torch.empty_like(x) if need_x else None
@@ -968,7 +969,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         with torch.cuda.device(x.device):
             ws = _class_loss_ws(lib.obman_class_loss_bwd_ws_bytes(_ct.addressof(p), int(need_x), int(need_w), int(need_b)),
                                 "obman_class_loss_bwd_ws_bytes", x.device)
-            _lib.check(lib.obman_class_loss_bwd(_ct.addressof(p), lse.data_ptr(), norm.data_ptr(), g_loss.data_ptr(), ws.data_ptr(), _ptr(dx),
+            _lib.check(lib.obman_class_loss_bwd(_ct.addressof(p), keep.data_ptr(), lse.data_ptr(), norm.data_ptr(), g_loss.data_ptr(), ws.data_ptr(), _ptr(dx),
                                                 _ptr(dw), _ptr(db), _stream()), "obman_class_loss_bwd")
         return dx, dw, db, None, None, None
 
