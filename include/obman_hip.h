@@ -297,21 +297,21 @@ int obman_bf16_shadow(const float* src, uint16_t* dst, long n, obman_stream_t st
  * nothing, whatever their x holds; another target outside [0, classes) makes the row's loss and every gradient NaN.
  * reduction: 0 per row, 1 sum, 2 mean over the rows that are not ignored (0 if there are none).
  * rows, classes: at most 2^22; width: at most 16384.
- * Forward: loss (rows floats, or one).  keep (obman_class_loss_keep_bytes: both operands as the products read them), lse [rows] and norm
- * (one float: 1, or 1 / rows kept) are what the backward pass needs; it does not read x and w again.
- * Backward: g_loss (rows floats, or one); dx, dw, db of the inputs' type, each may be NULL.  The gradient of the logits exists for a
- * piece of the classes at a time, in the scratch.  Fixed summation order: the same bits every call. */
+ * Forward: loss (rows floats, or one).  keep holds what the backward pass needs - it does not read x and w again; NULL (keeps = 0
+ * for the sizes): none will follow, and up to 32 rows are then scored with one read of w as it is.
+ * Backward: g_loss (rows floats, or one); dx, dw, db of the inputs' type, each may be NULL (need_* = 0 for the sizes).  The gradient
+ * of the logits exists for a piece of the classes at a time, in the scratch.  Fixed summation order: the same bits every call.
+ * obman_class_loss_sizes: bytes of keep and of the two calls' scratch ws, 256-byte aligned device memory. */
 typedef struct obman_class_loss_params {
   const void *x, *w, *bias, *target;
   long rows, classes, ignore_index;
   int width, type, target_wide, reduction;
 } obman_class_loss_params;
-long obman_class_loss_keep_bytes(const obman_class_loss_params* p);
-long obman_class_loss_fwd_ws_bytes(const obman_class_loss_params* p);
-int obman_class_loss_fwd(const obman_class_loss_params* p, void* keep, void* ws, float* loss, float* lse, float* norm, obman_stream_t stream);
-long obman_class_loss_bwd_ws_bytes(const obman_class_loss_params* p, int need_x, int need_w, int need_b);
-int obman_class_loss_bwd(const obman_class_loss_params* p, const void* keep, const float* lse, const float* norm, const float* g_loss,
-                         void* ws, void* dx, void* dw, void* db, obman_stream_t stream);
+int obman_class_loss_sizes(const obman_class_loss_params* p, int keeps, int need_x, int need_w, int need_b, long* keep_bytes,
+                           long* fwd_bytes, long* bwd_bytes);
+int obman_class_loss_fwd(const obman_class_loss_params* p, void* keep, void* ws, float* loss, obman_stream_t stream);
+int obman_class_loss_bwd(const obman_class_loss_params* p, const void* keep, const float* g_loss, void* ws, void* dx, void* dw,
+                         void* db, obman_stream_t stream);
 
 /* ---- K16: the gradient norm over a list of tensors, clipping, and the clipped optimizer step -----
  * norm = (sum |g|^p)^(1/p) over all elements of all tensors (norm: 2 = L2, 1 = L1, 0 = largest |g|); clipping multiplies every

@@ -46,11 +46,9 @@ _SIGNATURES = {
     "obman_imgstream_ws_bytes": (_c_long, "iii"),
     "obman_imgstream_fwd": (_c_int, "piiip" "ii" "iii" "pp" "pp" "p"),
     "obman_adam_step": (_c_int, "pi" "ddddd" "p"),
-    "obman_class_loss_fwd_ws_bytes": (_c_long, "p"),
-    "obman_class_loss_keep_bytes": (_c_long, "p"),
-    "obman_class_loss_fwd": (_c_int, "ppp" "ppp" "p"),
-    "obman_class_loss_bwd_ws_bytes": (_c_long, "p" "iii"),
-    "obman_class_loss_bwd": (_c_int, "ppppp" "p" "ppp" "p"),
+    "obman_class_loss_sizes": (_c_int, "p" "iiii" "ppp"),
+    "obman_class_loss_fwd": (_c_int, "pppp" "p"),
+    "obman_class_loss_bwd": (_c_int, "pppp" "ppp" "p"),
     "obman_grad_norm_ws_doubles": (_c_long, "i"),
     "obman_grad_norm": (_c_int, "pppi" "i" "pp" "p"),
     "obman_grad_clip": (_c_int, "pppi" "if" "pp" "p"),

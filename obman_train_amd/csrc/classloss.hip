@@ -15,6 +15,8 @@
 // size, before sums of many rows or classes) costs as much again as rounding the result.
 //
 // Rows that are ignored take no part: their x (which may be garbage) is packed as zeros, their g is zero.
+#include <cmath>
+
 #include "common.h"
 #include "../../include/obman_hip.h"
 
@@ -31,6 +33,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 typedef u16 u16x8u __attribute__((ext_vector_type(8), aligned(2)));
 typedef u16 u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned u32x4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 enum { F32 = 0, BF16 = 1, F16 = 2 };
@@ -39,11 +42,14 @@ enum { F32 = 0, BF16 = 1, F16 = 2 };
 // 32 rows of 8 blocks - is read in runs of 1 KB or more.  (Row-major, a step reads 64 of each row's bytes, half cache lines: the path
 // from L2 to LDS then holds the products at 900 Tflop/s; without any such reads they run at 1170 - 1270.)  Rows are padded with zeros
 // to whole tiles, so no address leaves an operand.
-constexpr int BI = 256, BJ = 128, BK = 32;  // tile: 256 x 128, four waves of 128 x 64; 72 KB of LDS, so two blocks share a CU and one's
-constexpr int STAGES = 3;                    // epilogue runs beside the other's products
+// Tile 256 x 128, four waves of 128 x 64.  72 KB of LDS, so two blocks share a CU and one's epilogue and waits run under the other's
+// products.  (256 x 256 with eight waves, four steps deep, one block on a CU, fetches a third less; at 19 200 x 64 050 x 512 it
+// measured 1 474 us for the forward product against 1 330, 328 against 304 for g, 290 against 300 and 250 against 253 for the other two.)
+constexpr int BI = 256, BJ = 128, BK = 32, WAVES = 4, STAGES = 3;
+constexpr int A_BYTES = BI * BK * 2, STAGE_BYTES = A_BYTES + BJ * BK * 2;
+constexpr int BIAS_AT = STAGES * STAGE_BYTES, LDS_BYTES = BIAS_AT + BI * 4;
+constexpr int SLOTS = 512;  // blocks that run at a time
 constexpr long MOST_ROWS = 1L << 22;         // of an operand: eight blocks of its columns stay within 32-bit offsets
-constexpr int A_BYTES = BI * BK * 2, B_BYTES = BJ * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int LDS_BYTES = STAGES * STAGE_BYTES + BI * 4;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float G_SCALE = 16384.f;  // |g| / max|c| <= 1 in fp16
 
@@ -55,8 +61,8 @@ struct Gemm {
   Side a, b;
   long ni, nj;      // extents of the result
   long k;           // contraction, a multiple of 32
-  long k_split;     // of it per block row of the grid's second axis
-  int ti, tj;       // tiles
+  long k_part;      // of it per part
+  int ti, tj, parts; // tiles, and parts of the contraction
   int na, nb;       // column blocks of a / b (an operand whose rows are contracted: tiles that run over its columns repeat the last block)
 };
 
@@ -71,7 +77,7 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, unsigned lds, un
 // whole rows at a time and need no swizzle.
 template <bool KR, int R>
 struct Operand {
-  static constexpr int N = R * BK * 2 / 1024 / 4;  // wave-wide loads of 1 KB per wave and step
+  static constexpr int N = R * BK * 2 / 1024 / WAVES;  // wave-wide loads of 1 KB per wave and step
   const u16* base;  // at the next step's k
   long step;
   unsigned voff[N];
@@ -148,11 +154,13 @@ __device__ __forceinline__ long target_of(const void* t, int wide, long r) {
   return wide ? static_cast<const long*>(t)[r] : (long)static_cast<const int*>(t)[r];
 }
 
-// Consecutive ids of one XCD (ids go round the eight) take consecutive tiles; tiles run 8 j wide, so that what an XCD's CUs work on
-// at a time (8 x 8 tiles: 3 MB of operands at width 512) stays in its 4 MB L2.
-__device__ __forceinline__ void tile_of(const Gemm& g, int& i, int& j) {
-  const int n = g.ti * g.tj, id = blockIdx.x, x = id & 7, q = n >> 3, rem = n & 7;
-  const int v = x * q + (x < rem ? x : rem) + (id >> 3);
+// Consecutive ids of one XCD (ids go round the eight) take consecutive tiles of one part of the contraction; tiles run 8 j wide, so
+// that what an XCD's CUs work on at a time (8 x 8 tiles: 3 MB of operands at width 512) stays in its 4 MB L2.
+__device__ __forceinline__ void tile_of(const Gemm& g, int id, int& i, int& j, int& part) {
+  const int tiles = g.ti * g.tj, n = tiles * g.parts, x = id & 7, q = n >> 3, rem = n & 7;
+  int v = x * q + (x < rem ? x : rem) + (id >> 3);
+  part = v / tiles;
+  v -= part * tiles;
   const int per = 8 * g.ti, group = v / per, in = v - group * per;
   const int w = g.tj - group * 8 < 8 ? g.tj - group * 8 : 8;
   i = in / w;
@@ -169,7 +177,7 @@ struct Scale {
 struct Ctx {
   long i0, j0;
   int wi, wj, lane, tid, ti_index, tj_index, split;
-  char* smem;
+  char *smem, *bias;
 };
 
 __device__ __forceinline__ void clear(f32x16 (&acc)[4][2]) {
@@ -190,14 +198,14 @@ struct Bias {
   int type;
   long class0, classes;
   __device__ __forceinline__ static const float* mine(const Ctx& c) {  // of this lane's classes: 8 q + 0 .. 3 from here on
-    return reinterpret_cast<const float*>(c.smem + STAGES * STAGE_BYTES) + c.wi * 128 + 4 * (c.lane >> 5);
+    return reinterpret_cast<const float*>(c.bias) + c.wi * 128 + 4 * (c.lane >> 5);
   }
   __device__ __forceinline__ void before(const Ctx& c, f32x16 (&acc)[4][2]) const {
     const long v0 = class0 + c.i0;
     const bool plain = !bias && v0 + BI <= classes;
     if (SPLIT || !plain) {
       const long v = v0 + c.tid;
-      reinterpret_cast<float*>(c.smem + STAGES * STAGE_BYTES)[c.tid] = v >= classes ? -INFINITY : bias ? load_one(bias, type, v) : 0.f;
+      reinterpret_cast<float*>(c.bias)[c.tid] = v >= classes ? -INFINITY : bias ? load_one(bias, type, v) : 0.f;
     }
     if (SPLIT || plain) {
       clear(acc);
@@ -310,7 +318,7 @@ template <int T, bool SPLIT>
 struct Grad {
   Bias<SPLIT> bias;
   const RowConst* rows;
-  long rows_padded;
+  long n_rows, rows_padded;
   u16* out;
   long plane;
   int columns;      // of out
@@ -322,7 +330,7 @@ struct Grad {
     for (int fj = 0; fj < 2; ++fj) {
       const long r = c.j0 + c.wj * 64 + fj * 32 + (c.lane & 31);
       RowConst k = {INFINITY, 0.f, -1, 0};
-      if (r < g.nj) k = rows[r];
+      if (r < n_rows) k = rows[r];
       const int t = target_at(k.target, bias.class0 + c.i0 + c.wi * 128, c.lane);
 #pragma unroll
       for (int fi = 0; fi < 4; ++fi)
@@ -424,14 +432,14 @@ struct Slab {
 
 // C[i, j] = sum_k A(i, k) B(j, k); TERMS = 3: both operands in two planes
 template <bool A_KR, bool B_KR, int T, int TERMS, class Epi>
-__global__ __launch_bounds__(256, 2) void gemm_kernel(Gemm g, Epi epi) {
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
+__device__ __forceinline__ void gemm(const Gemm& g, const Epi& epi, int id, char* smem) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int bi, bj;
-  tile_of(g, bi, bj);
+  int bi, bj, part;
+  tile_of(g, id, bi, bj, part);
   bi = __builtin_amdgcn_readfirstlane(bi);
   bj = __builtin_amdgcn_readfirstlane(bj);
-  const Ctx ctx{(long)bi * BI, (long)bj * BJ, wave & 1, wave >> 1, lane, tid, bi, bj, (int)blockIdx.y, smem};
+  part = __builtin_amdgcn_readfirstlane(part);
+  const Ctx ctx{(long)bi * BI, (long)bj * BJ, wave & 1, wave >> 1, lane, tid, bi, bj, part, smem, smem + BIAS_AT};
   Operand<A_KR, BI> oa;
   Operand<B_KR, BJ> ob;
   oa.init(g.a, bi * (BI / 32), g.na, wave, lane);
@@ -440,7 +448,7 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(Gemm g, Epi epi) {
   Frag<B_KR> fb;
   fa.init(ctx.wi * 128, lane);
   fb.init(ctx.wj * 64, lane);
-  const long kb = (long)blockIdx.y * g.k_split, ke = kb + g.k_split < g.k ? kb + g.k_split : g.k;
+  const long kb = part * g.k_part, ke = kb + g.k_part < g.k ? kb + g.k_part : g.k;
   const int steps = ke > kb ? (int)((ke - kb) / BK) * TERMS : 0;
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
 
@@ -464,38 +472,60 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(Gemm g, Epi epi) {
       start();
     }
   };
-  constexpr int PER = Operand<A_KR, BI>::N + Operand<B_KR, BJ>::N;
-  static_assert(PER == 6, "the counted wait below");
+  const char* from = smem;
+  const auto next = [&](const char* p) { return p == smem + (STAGES - 1) * STAGE_BYTES ? smem : p + STAGE_BYTES; };
+  const auto read = [&](const char* p, int ks, u32x4 (&a)[4], u32x4 (&b)[2]) {
+#pragma unroll
+    for (int f = 0; f < 2; ++f) b[f] = fb.read(p + A_BYTES, f, ks);
+#pragma unroll
+    for (int f = 0; f < 4; ++f) a[f] = fa.read(p, f, ks);
+  };
+  const auto products = [&](const u32x4 (&a)[4], const u32x4 (&b)[2]) {
+    __builtin_amdgcn_sched_barrier(0);  // the reads before go out first
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int f = 0; f < 4; ++f)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) acc[f][h] = mfma<T>(a[f], b[h], acc[f][h]);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  static_assert(Operand<A_KR, BI>::N + Operand<B_KR, BJ>::N == 6, "the counted wait below");
+  u32x4 a0[4], b0[2], a1[4], b1[2];
   if (steps > 0) issue();
   if (steps > 1) issue();
-  const char* from = smem;
   for (int s = 0; s < steps; ++s) {
     // step s has arrived for every wave (only step s + 1 may still be under way), and every wave has read step s - 1, whose slot is next
     if (s + 1 < steps) asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    u32x4 a[2][4], b[2][2];
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-#pragma unroll
-      for (int f = 0; f < 2; ++f) b[ks][f] = fb.read(from + A_BYTES, f, ks);
-#pragma unroll
-      for (int f = 0; f < 4; ++f) a[ks][f] = fa.read(from, f, ks);
-    }
+    read(from, 0, a0, b0);
+    read(from, 1, a1, b1);
     if (s + 2 < steps) issue();
-    from = from == smem + (STAGES - 1) * STAGE_BYTES ? smem : from + STAGE_BYTES;
-    __builtin_amdgcn_sched_barrier(0);  // all reads go out before the first product waits for one
-    __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int f = 0; f < 4; ++f)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) acc[f][h] = mfma<T>(a[ks][f], b[ks][h], acc[f][h]);
-    __builtin_amdgcn_s_setprio(0);
-    __builtin_amdgcn_sched_barrier(0);
+    from = next(from);
+    products(a0, b0);
+    products(a1, b1);
   }
   __syncthreads();
   epi.after(g, ctx, acc);
+}
+
+template <int T, int TERMS, class Epi>
+__global__ __launch_bounds__(WAVES * 64, 2) void logits_kernel(Gemm g, Epi epi) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  gemm<false, false, T, TERMS>(g, epi, blockIdx.x, smem);
+}
+
+// dx and dw of a piece of the classes in one launch (each may have no blocks): both read the same g, and their blocks fill each
+// other's last round.  The longer ones come first; first: how many blocks that is, rounded up to whole rounds of the XCDs.
+template <int T, int TERMS>
+__global__ __launch_bounds__(WAVES * 64, 2) void grads_kernel(Gemm gx, Slab ex, int nx, Gemm gw, Slab ew, int nw, int x_first) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int first = ((x_first ? nx : nw) + 7) & ~7;
+  const bool is_x = ((int)blockIdx.x < first) == (x_first != 0);
+  const int id = (int)blockIdx.x < first ? blockIdx.x : blockIdx.x - first;
+  if (id >= (is_x ? nx : nw)) return;
+  if (is_x) gemm<true, false, T, TERMS>(gx, ex, id, smem);
+  else gemm<true, true, T, TERMS>(gw, ew, id, smem);
 }
 
 // ------------------------------------------------------------------------------------------------------- operands and rows
@@ -598,51 +628,204 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack px, Pack pw, int width, 
   }
 }
 
-// per row: join over the tiles of classes; loss per row, and per block of rows the sum of losses and the number of kept rows
-__global__ __launch_bounds__(256) void join_rows_kernel(const float2* __restrict__ part, int tiles, long rows, long classes, const float* __restrict__ picked,
-                                                       const void* target, int wide, long ignore, float* __restrict__ lse, float* __restrict__ loss,
-                                                       double2* __restrict__ sums) {
-  // 64 rows a block, four threads a row
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const long r = (long)blockIdx.x * 64 + lane;
-  __shared__ float2 red[4][64];
-  float m = -INFINITY, s = 0.f;
-  if (r < rows)
-    for (int t = w; t < tiles; t += 4) {
-      const float2 p = part[(long)t * rows + r];
-      const float top = fmaxf(m, p.x), ref = top == -INFINITY ? 0.f : top * LOG2E;
-      s = s * __builtin_amdgcn_exp2f(m * LOG2E - ref) + p.y * __builtin_amdgcn_exp2f(p.x * LOG2E - ref);
-      m = top;
-    }
-  red[w][lane] = make_float2(m, s);
-  __syncthreads();
-  if (w) return;
-  double l = 0.0, kept = 0.0;
-  if (r < rows) {
+// Few rows (scoring single features): the table is read once, as it is, and that read is the time.  A wave holds 32 classes x up to 32
+// rows: its lanes load 16 bytes of each of the 32 class rows straight into matrix operands (a lane's element order along the width is
+// free as long as x, staged in LDS, has the same), fp32 on the fp32 instruction.  Blocks run over the table with running statistics.
+constexpr int FEW = 32;
+template <int TYPE> struct FewT { static constexpr int E = 8; };  // elements of a 16-byte piece
+template <> struct FewT<F32> { static constexpr int E = 4; };
+template <int TYPE>
+__global__ __launch_bounds__(256) void few_kernel(const void* __restrict__ xs, const void* __restrict__ ws, const void* __restrict__ bias, const void* target, int wide, int rows,
+                                                 long classes, int width, float2* __restrict__ part, float* __restrict__ picked) {
+  constexpr int E = FewT<TYPE>::E, SIZE = 16 / E, AHEAD = 8;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ float2 red[4][FEW];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int pieces = (width + 2 * E - 1) / (2 * E);  // of 2 E columns, one 16-byte half for each half of the wave
+  // x in LDS: [piece][half][row] 16 bytes, zeros behind the width and the last row
+  for (int i = tid; i < pieces * 2 * FEW; i += 256) {
+    const int r = i % FEW, c = i / FEW * E;
+    u32x4 v = {0, 0, 0, 0};
+    if (r < rows) {
+      const char* p = static_cast<const char*>(xs) + ((long)r * width + c) * SIZE;
+      if (c + E <= width) v = *reinterpret_cast<const u32x4u*>(p);
+      else
 #pragma unroll
-    for (int k = 1; k < 4; ++k) {
-      const float2 p = red[k][lane];
-      const float top = fmaxf(m, p.x), ref = top == -INFINITY ? 0.f : top * LOG2E;
-      s = s * __builtin_amdgcn_exp2f(m * LOG2E - ref) + p.y * __builtin_amdgcn_exp2f(p.x * LOG2E - ref);
-      m = top;
+        for (int e = 0; e < E; ++e) {
+          if (c + e >= width) continue;
+          if constexpr (TYPE == F32) v[e] = reinterpret_cast<const unsigned*>(p)[e];
+          else v[e >> 1] |= (unsigned)reinterpret_cast<const u16*>(p)[e] << (16 * (e & 1));
+        }
     }
-    const long t = target_of(target, wide, r);
-    float z = m + LN2 * __builtin_amdgcn_logf(s);  // v_log_f32: log2
-    if (t != ignore && (t < 0 || t >= classes)) z = NAN;  // a label outside the table poisons the loss instead of being read
-    lse[r] = z;
-    const float row = t == ignore ? 0.f : z - (t >= 0 && t < classes ? picked[r] : 0.f);
-    if (loss) loss[r] = row;
-    l = row;
-    kept = t != ignore;
+    reinterpret_cast<u32x4*>(smem)[i] = v;
   }
-  if (sums) {
+  __syncthreads();
+  const char* xl = smem + (half * FEW + (lane & 31)) * 16;
+  const int r = lane & 31;
+  const long t = r < rows ? target_of(target, wide, r) : -1;
+  const int safe = width / (2 * E);  // pieces that lie inside the row
+  float m = -INFINITY, s = 0.f;
+  for (long v0 = ((long)blockIdx.x * 4 + wave) * 32; v0 < classes; v0 += (long)gridDim.x * 128) {
+    const long v = v0 + (lane & 31);
+    const char* row = static_cast<const char*>(ws) + (v < classes ? v : classes - 1) * width * SIZE + half * 16;
+    f32x16 acc;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) { l += __shfl_xor(l, off, 64); kept += __shfl_xor(kept, off, 64); }
-    if (lane == 0) sums[blockIdx.x] = make_double2(l, kept);
+    for (int q = 0; q < 16; ++q) acc[q] = 0.f;
+    const auto step = [&](u32x4 a, int p) {
+      const u32x4 b = *reinterpret_cast<const u32x4*>(xl + p * (2 * FEW * 16));
+      if constexpr (TYPE == F32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(b[e]), acc, 0, 0, 0);
+      } else acc = mfma<TYPE>(a, b, acc);
+    };
+    int p = 0;
+    for (; p + AHEAD <= safe; p += AHEAD) {
+      u32x4 a[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) a[u] = *reinterpret_cast<const u32x4u*>(row + (p + u) * 32);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) step(a[u], p + u);
+    }
+    for (; p < safe; ++p) step(*reinterpret_cast<const u32x4u*>(row + p * 32), p);
+    if (p < pieces) {
+      u32x4 a = {0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int c = p * 2 * E + half * E + e;
+        if (c >= width) continue;
+        if constexpr (TYPE == F32) a[e] = reinterpret_cast<const unsigned*>(row + p * 32)[e];
+        else a[e >> 1] |= (unsigned)reinterpret_cast<const u16*>(row + p * 32)[e] << (16 * (e & 1));
+      }
+      step(a, p);
+    }
+    // lane: row lane % 32, classes v0 + 8 (q / 4) + 4 half + q % 4
+    float top = m;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+      const long c = v0 + 8 * (q >> 2) + 4 * half + (q & 3);
+      acc[q] = c < classes ? acc[q] + (bias ? load_one(bias, TYPE, c) : 0.f) : -INFINITY;
+      if (c == t) picked[r] = acc[q];
+      top = fmaxf(top, acc[q]);
+    }
+    const float ref = top == -INFINITY ? 0.f : top * LOG2E;
+    s *= __builtin_amdgcn_exp2f(m * LOG2E - ref);
+#pragma unroll
+    for (int q = 0; q < 16; ++q) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[q], LOG2E, -ref));
+    m = top;
+  }
+  const auto join = [&](float m2, float s2) {
+    const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top * LOG2E;
+    s = s * __builtin_amdgcn_exp2f(m * LOG2E - ref) + s2 * __builtin_amdgcn_exp2f(m2 * LOG2E - ref);
+    m = top;
+  };
+  join(__shfl_xor(m, 32, 64), __shfl_xor(s, 32, 64));
+  if (half == 0) red[wave][r] = make_float2(m, s);
+  __syncthreads();
+  if (wave == 0 && half == 0 && r < rows) {
+#pragma unroll
+    for (int w = 1; w < 4; ++w) join(red[w][r].x, red[w][r].y);
+    part[(long)r * gridDim.x + blockIdx.x] = make_float2(m, s);
   }
 }
 
+// a row's loss from its log-sum-exp
+__device__ __forceinline__ float row_loss(float lse, long t, long classes, long ignore, const float* picked, long r) {
+  return t == ignore ? 0.f : lse - (t >= 0 && t < classes ? picked[r] : 0.f);
+}
 // loss = sum or mean over the kept rows (no row kept: 0); norm = what a row's gradient is multiplied by
+__device__ __forceinline__ void total_loss(double l, double k, int mean, float* loss, float* norm) {
+  if (k < 1.0) k = 1.0;
+  *loss = (float)(mean ? l / k : l);
+  *norm = (float)(mean ? 1.0 / k : 1.0);
+}
+
+// the end of few_kernel: a wave joins a row's block statistics, one block everything
+__global__ __launch_bounds__(1024) void few_join_kernel(const float2* __restrict__ part, int n, int rows, long classes, const float* __restrict__ picked, const void* target, int wide,
+                                                       long ignore, int reduction, float* __restrict__ loss, float* __restrict__ lse, float* __restrict__ norm) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ double2 red[FEW];
+  for (int r = wave; r < rows; r += 16) {
+    float m = -INFINITY, s = 0.f;
+    const auto join = [&](float m2, float s2) {
+      const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top * LOG2E;
+      s = s * __builtin_amdgcn_exp2f(m * LOG2E - ref) + s2 * __builtin_amdgcn_exp2f(m2 * LOG2E - ref);
+      m = top;
+    };
+    for (int i = lane; i < n; i += 64) { const float2 p = part[(long)r * n + i]; join(p.x, p.y); }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) join(__shfl_xor(m, off, 64), __shfl_xor(s, off, 64));
+    const long t = target_of(target, wide, r);
+    float z = m + LN2 * __builtin_amdgcn_logf(s);
+    if (t != ignore && (t < 0 || t >= classes)) z = NAN;
+    const float l = row_loss(z, t, classes, ignore, picked, r);
+    if (lane == 0) {
+      lse[r] = z;
+      if (reduction == 0) loss[r] = l;
+      red[r] = make_double2(l, t != ignore);
+    }
+  }
+  if (reduction == 0) return;
+  __syncthreads();
+  if (threadIdx.x) return;
+  double l = 0.0, k = 0.0;
+  for (int r = 0; r < rows; ++r) { l += red[r].x; k += red[r].y; }
+  total_loss(l, k, reduction == 2, loss, norm);
+}
+
+// Per row: join over the tiles of classes; loss per row, what the backward pass needs of the row if every row weighs the same, and per
+// block of 64 rows the sum of losses and the number of kept rows.  WHOLE: one block does all rows and the reduction.
+template <bool WHOLE>
+__global__ __launch_bounds__(WHOLE ? 1024 : 256) void join_rows_kernel(const float2* __restrict__ part, int tiles, long rows, long classes, const float* __restrict__ picked,
+                                                                      const void* target, int wide, long ignore, int reduction, float g_scale, float* __restrict__ lse,
+                                                                      float* __restrict__ loss, RowConst* __restrict__ consts, double2* __restrict__ sums, float* __restrict__ norm) {
+  constexpr int GROUPS = WHOLE ? 4 : 1;  // of 64 rows x 4 threads
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave & 3, group = wave >> 2;
+  __shared__ float2 red[GROUPS][4][64];
+  double l = 0.0, kept = 0.0;
+  for (long r0 = (long)blockIdx.x * 64; r0 < rows; r0 += WHOLE ? 256 : rows) {  // (not WHOLE: once)
+    const long r = r0 + group * 64 + lane;
+    float m = -INFINITY, s = 0.f;
+    const auto join = [&](float2 p) {
+      const float top = fmaxf(m, p.x), ref = top == -INFINITY ? 0.f : top * LOG2E;
+      s = s * __builtin_amdgcn_exp2f(m * LOG2E - ref) + p.y * __builtin_amdgcn_exp2f(p.x * LOG2E - ref);
+      m = top;
+    };
+    if (r < rows)
+      for (int t = w; t < tiles; t += 4) join(part[(long)t * rows + r]);
+    red[group][w][lane] = make_float2(m, s);
+    __syncthreads();
+    if (w == 0 && r < rows) {
+#pragma unroll
+      for (int k = 1; k < 4; ++k) join(red[group][k][lane]);
+      const long t = target_of(target, wide, r);
+      float z = m + LN2 * __builtin_amdgcn_logf(s);  // v_log_f32: log2
+      if (t != ignore && (t < 0 || t >= classes)) z = NAN;  // a label outside the table poisons the loss instead of being read
+      lse[r] = z;
+      const float row = row_loss(z, t, classes, ignore, picked, r);
+      if (reduction == 0) loss[r] = row;
+      if (consts) {
+        const bool none = t == ignore;
+        consts[r] = RowConst{none ? INFINITY : z * LOG2E - log2f(g_scale), none ? 0.f : g_scale, none || t < 0 || t >= classes ? -1 : (int)t, 0};
+      }
+      l += row;
+      kept += t != ignore;
+    }
+    __syncthreads();
+  }
+  if (reduction == 0) return;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) { l += __shfl_xor(l, off, 64); kept += __shfl_xor(kept, off, 64); }
+  if constexpr (!WHOLE) {
+    if (threadIdx.x == 0) sums[blockIdx.x] = make_double2(l, kept);
+  } else {
+    __shared__ double2 total[GROUPS];
+    if (w == 0 && lane == 0) total[group] = make_double2(l, kept);
+    __syncthreads();
+    if (threadIdx.x == 0)
+      total_loss((total[0].x + total[1].x) + (total[2].x + total[3].x), (total[0].y + total[1].y) + (total[2].y + total[3].y), reduction == 2, loss, norm);
+  }
+}
+
 __global__ __launch_bounds__(256) void reduce_kernel(const double2* __restrict__ sums, int n, int mean, float* __restrict__ loss, float* __restrict__ norm) {
   double l = 0.0, k = 0.0;
   for (int i = threadIdx.x; i < n; i += 256) { const double2 p = sums[i]; l += p.x; k += p.y; }
@@ -654,82 +837,81 @@ __global__ __launch_bounds__(256) void reduce_kernel(const double2* __restrict__
   if (threadIdx.x) return;
   l = (red[0][0] + red[0][1]) + (red[0][2] + red[0][3]);
   k = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-  if (k < 1.0) k = 1.0;
-  *loss = (float)(mean ? l / k : l);
-  *norm = (float)(mean ? 1.0 / k : 1.0);
+  total_loss(l, k, mean, loss, norm);
 }
 
-// backward constants: RowConst per row and alpha, the factor of every result.  g_loss: one value (sum, mean) or one per row, scaled
-// here to at most 1 in magnitude by a power of two that alpha takes back
+// A gradient for every row: RowConst with its weight, scaled to at most 1 in magnitude by a power of two; alpha takes it back.
 __global__ __launch_bounds__(1024) void rows_kernel(const float* __restrict__ lse, const void* target, int wide, long ignore, long rows, const float* __restrict__ g_loss,
-                                                   int per_row, const float* __restrict__ norm, float g_scale, RowConst* __restrict__ out, float* __restrict__ alpha) {
+                                                   float g_scale, RowConst* __restrict__ out, float* __restrict__ alpha) {
   float top = 0.f;
   __shared__ float red[16];
-  if (per_row) {  // every block finds the same maximum
-    for (long r = threadIdx.x; r < rows; r += 1024) {
-      const float a = fabsf(g_loss[r]);
-      if (a > top && a < INFINITY && target_of(target, wide, r) != ignore) top = a;
-    }
-    top = obman_wave_max(top);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
-    __syncthreads();
-    top = red[0];
-#pragma unroll
-    for (int w = 1; w < 16; ++w) top = fmaxf(top, red[w]);
+  for (long r = threadIdx.x; r < rows; r += 1024) {  // every block finds the same maximum
+    const float a = fabsf(g_loss[r]);
+    if (a > top && a < INFINITY && target_of(target, wide, r) != ignore) top = a;
   }
+  top = obman_wave_max(top);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+  __syncthreads();
+  top = red[0];
+#pragma unroll
+  for (int w = 1; w < 16; ++w) top = fmaxf(top, red[w]);
   int e = 0;
   if (top > 0.f) (void)frexpf(top, &e);
   e = e > 120 ? 120 : e < -120 ? -120 : e;
   const float up = ldexpf(1.f, e), down = ldexpf(1.f, -e);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *alpha = per_row ? up / g_scale : *g_loss * *norm / g_scale;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *alpha = up;
   const long r = (long)blockIdx.x * 1024 + threadIdx.x;
   if (r >= rows) return;
   const long t = target_of(target, wide, r);
-  RowConst k;
-  const float w = t == ignore ? 0.f : (per_row ? g_loss[r] * down : 1.f) * g_scale;
-  k.c = w;
-  k.lse2 = w == 0.f ? INFINITY : lse[r] * LOG2E - log2f(fabsf(w));
-  k.target = w == 0.f || t < 0 || t > 0x7fffffffL ? -1 : (int)t;
-  k.pad = 0;
-  out[r] = k;
+  const float w = t == ignore ? 0.f : g_loss[r] * down * g_scale;
+  out[r] = RowConst{w == 0.f ? INFINITY : lse[r] * LOG2E - log2f(fabsf(w)), w, w == 0.f || t < 0 || t > 0x7fffffffL ? -1 : (int)t, 0};
 }
 
-// sum of the slabs times alpha into the gradient's own type
-__global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ slabs, int n, long slab, long rows, int ld, int width, const float* __restrict__ alpha,
-                                                    const float* __restrict__ scale, void* __restrict__ out, int type) {
-  const float k = *alpha * (scale ? 1.f / *scale : 1.f);
+// The end of a piece: the slabs' sums times alpha in the gradient's own type (x: grid row 0, w: 1), and the bias gradient from the
+// column sums of the tiles of rows, in order (2).  rows = 0: nothing to do.  alpha = *alpha[0] * *alpha[1] / g_scale.
+struct Finish { const float* slabs; int n; long slab, rows; const float* scale; void* out; };
+struct FinishBias { const float* sums; int n, columns; long classes; void* out; };
+struct Alpha {
+  const float *a, *b;
+  float over;
+  __device__ __forceinline__ float value() const { return *a * (b ? *b : 1.f) * over; }
+};
+__global__ __launch_bounds__(256) void finish_kernel(Finish fx, Finish fw, FinishBias fb, int ld, int width, Alpha alpha, int type) {
+  if (blockIdx.y == 2) {
+    const float k = alpha.value();
+    for (long v = (long)blockIdx.x * 256 + threadIdx.x; v < fb.classes; v += (long)gridDim.x * 256) {
+      double s = 0.0;
+      for (int t = 0; t < fb.n; ++t) s += fb.sums[(long)t * fb.columns + v];
+      store_one(fb.out, type, v, (float)(s * k));
+    }
+    return;
+  }
+  const Finish f = blockIdx.y == 0 ? fx : fw;
   const int per = (width + 3) >> 2;
-  const long total = rows * per;
+  const long total = f.rows * per;
+  if ((long)blockIdx.x * 256 >= total) return;
+  const float k = alpha.value() * (f.scale ? 1.f / *f.scale : 1.f);
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
     const long r = i / per;
     const int c = (int)(i - r * per) * 4;
-    const float* p = slabs + r * ld + c;
+    const float* p = f.slabs + r * ld + c;
     f32x4 v = *reinterpret_cast<const f32x4*>(p);
-    for (int s = 1; s < n; ++s) v += *reinterpret_cast<const f32x4*>(p + s * slab);
+    for (int s = 1; s < f.n; ++s) v += *reinterpret_cast<const f32x4*>(p + s * f.slab);
     const long at = r * width + c;
     if (c + 4 <= width) {
-      if (type == F32) *reinterpret_cast<f32x4u*>(static_cast<float*>(out) + at) = f32x4u{v[0] * k, v[1] * k, v[2] * k, v[3] * k};
+      if (type == F32) *reinterpret_cast<f32x4u*>(static_cast<float*>(f.out) + at) = f32x4u{v[0] * k, v[1] * k, v[2] * k, v[3] * k};
       else {
         u16x4u o;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = type == BF16 ? narrow<BF16>(v[e] * k) : narrow<F16>(v[e] * k);
-        *reinterpret_cast<u16x4u*>(static_cast<u16*>(out) + at) = o;
+        *reinterpret_cast<u16x4u*>(static_cast<u16*>(f.out) + at) = o;
       }
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (c + e < width) store_one(out, type, at + e, v[e] * k);
+        if (c + e < width) store_one(f.out, type, at + e, v[e] * k);
     }
   }
-}
-
-// the bias gradient: the column sums of the tiles of rows, in order
-__global__ __launch_bounds__(256) void bias_kernel(const float* __restrict__ sums, int n, int columns, long classes, const float* __restrict__ alpha, void* __restrict__ out, int type) {
-  const long v = (long)blockIdx.x * 256 + threadIdx.x;
-  if (v >= classes) return;
-  double s = 0.0;
-  for (int t = 0; t < n; ++t) s += sums[(long)t * columns + v];
-  store_one(out, type, v, (float)(s * *alpha));
 }
 
 // --------------------------------------------------------------------------------------------------------------- the calls
@@ -748,13 +930,14 @@ struct Carve {  // scratch: offsets first, pointers once a base is there
 };
 
 constexpr long PIECE_BYTES = 512L << 20;  // of g at a time
-constexpr int SLOTS = 512;                // blocks that run at a time: two per CU
 
-// what the forward pass leaves for the backward pass: both operands in blocks, and their scales
+// what the forward pass leaves for the backward pass: both operands in blocks, their scales, and per row the log-sum-exp and, if all
+// rows weigh the same, the constants
 struct Keep {
   Side x, w;
   u16 *xp, *wp;
-  float* scales;
+  float *scales, *lse, *norm;
+  RowConst* rows;
   int blocks;  // of 32 columns
   size_t bytes;
 };
@@ -765,13 +948,60 @@ static Keep keep_of(const obman_class_loss_params& p, void* mem) {
   const long xr = up(p.rows, BJ), wr = up(p.classes, BI);
   k.blocks = obman_cdiv(p.width, 32);
   const long xn = xr * k.blocks * 32, wn = wr * k.blocks * 32;
-  k.scales = c.take<float>(2);
+  k.scales = c.take<float>(4);
+  k.norm = k.scales + 2;
+  k.lse = c.take<float>(p.rows);
+  k.rows = c.take<RowConst>(p.reduction ? p.rows : 0);
   k.xp = c.take<u16>(xn * planes);
   k.wp = c.take<u16>(wn * planes);
   k.x = {k.xp, xn, xr};
   k.w = {k.wp, wn, wr};
   k.bytes = c.at;
   return k;
+}
+
+// dynamic LDS of a kernel, allowed once per device
+template <auto KERNEL, int BYTES>
+static hipError_t allow_lds() {
+  static std::atomic<unsigned> done{0};
+  const int dev = current_device();
+  if (done.load(std::memory_order_relaxed) >> dev & 1) return hipSuccess;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, BYTES);
+  if (e == hipSuccess) done.fetch_or(1u << dev, std::memory_order_relaxed);
+  return e;
+}
+
+// scoring of few rows: the table is read as it is
+constexpr int FEW_BLOCKS = 512;
+constexpr size_t FEW_LDS = 128 * 1024;  // of x: width 2048 in 16 bits, 1024 in fp32
+struct Few {
+  float2* part;
+  float *picked, *lse, *norm;
+  int blocks;
+  size_t bytes, lds;
+};
+static bool few_of(const obman_class_loss_params& p, void* mem, Few* o) {
+  Carve c{static_cast<char*>(mem)};
+  const long groups = (p.classes + 127) / 128;
+  o->blocks = (int)(groups < FEW_BLOCKS ? groups : FEW_BLOCKS);
+  o->part = c.take<float2>((size_t)o->blocks * FEW);
+  o->picked = c.take<float>(FEW);
+  o->lse = c.take<float>(FEW);
+  o->norm = c.take<float>(1);
+  o->bytes = c.at;
+  const int e = p.type == F32 ? 4 : 8;
+  o->lds = (size_t)up(p.width, 2 * e) / e * FEW * 16;
+  return p.rows <= FEW && o->lds <= FEW_LDS;
+}
+template <int TYPE>
+static int few(const obman_class_loss_params& p, const Few& o, float* loss, hipStream_t st) {
+  const hipError_t a = allow_lds<few_kernel<TYPE>, (int)FEW_LDS>();
+  if (a != hipSuccess) return (int)a;
+  few_kernel<TYPE><<<o.blocks, 256, o.lds, st>>>(p.x, p.w, p.bias, p.target, p.target_wide, (int)p.rows, p.classes, p.width, o.part, o.picked);
+  OBMAN_LAUNCH_CHECK();
+  few_join_kernel<<<1, 1024, 0, st>>>(o.part, o.blocks, (int)p.rows, p.classes, o.picked, p.target, p.target_wide, p.ignore_index, p.reduction, loss, o.lse, o.norm);
+  OBMAN_LAUNCH_CHECK();
+  return 0;
 }
 
 struct Forward {
@@ -795,36 +1025,43 @@ static Forward forward_of(const obman_class_loss_params& p, void* mem) {
   return o;
 }
 
-// Into how many parts the contraction is cut: the fewest step times of 32 over all rounds of the slots, a part costing START steps
-// more (its pipeline's start and its slab)
+// Into how many parts the contractions of dx and dw are cut: the least time of their common launch in steps of 32, a part costing
+// START steps more (its pipeline's start and its slab); the time is the whole rounds of the longer blocks, or all work spread over
+// the slots plus half a shorter block of unevenness.
 constexpr long START = 40;
-static int split_of(long tiles, long k) {
-  long best = 0;
-  int n = 1;
-  for (int c = 1; c <= 64; ++c) {
-    if (c > 1 && k / c < 256) break;
-    const long t = (tiles * c + SLOTS - 1) / SLOTS * (k / BK / c + START);
-    if (c == 1 || t < best) { best = t; n = c; }
+struct Parts { int x, w; bool x_first; };
+static Parts parts_of(long tiles_x, long k_x, long tiles_w, long k_w) {
+  Parts best{1, 1, true};
+  double least = 0.0;
+  for (int x = 1; x <= (tiles_x ? 32 : 1); ++x) {
+    if (x > 1 && k_x / x < 256) break;
+    for (int w = 1; w <= (tiles_w ? 32 : 1); ++w) {
+      if (w > 1 && k_w / w < 256) break;
+      const double lx = k_x / BK / x + START, lw = k_w / BK / w + START;
+      const bool first = !tiles_w || (tiles_x && lx >= lw);
+      const double nx = (double)tiles_x * x, nw = (double)tiles_w * w, n = first ? nx : nw, l = first ? lx : lw, shorter = tiles_x && tiles_w ? (first ? lw : lx) : l;
+      const double rounds = ceil(n / SLOTS) * l, spread = (nx * lx + nw * lw) / SLOTS + 0.5 * shorter;
+      const double t = rounds > spread ? rounds : spread;
+      if (least == 0.0 || t < least) { least = t; best = {x, w, first}; }
+    }
   }
-  return n;
+  return best;
 }
-static long split_len(long k, int n) { return up((k + n - 1) / n, BK); }
-
 struct Backward {
   RowConst* rows;
   float* alpha;
   u16* g;
   long g_plane, piece;
   float *dx_slabs, *dw_slabs, *sums;
-  int dx_split, dw_split;
+  Parts parts;
   size_t bytes;
 };
 static Backward backward_of(const obman_class_loss_params& p, const Keep& k, void* mem, bool need_x, bool need_w, bool need_b) {
   Carve c{static_cast<char*>(mem)};
   Backward o;
-  const int planes = p.type == F32 ? 2 : 1, ld = k.blocks * 32;
+  const int planes = p.type == F32 ? 2 : 1, terms = p.type == F32 ? 3 : 1, ld = k.blocks * 32;
   const long xr = k.x.rows, all = up(p.classes, 32);
-  o.rows = c.take<RowConst>(p.rows);
+  o.rows = c.take<RowConst>(p.reduction ? 0 : p.rows);
   o.alpha = c.take<float>(1);
   long most = PIECE_BYTES / (xr * 2 * planes) / BI * BI;
   if (most < 2 * BI) most = 2 * BI;
@@ -833,10 +1070,9 @@ static Backward backward_of(const obman_class_loss_params& p, const Keep& k, voi
   if (o.piece > all) o.piece = all;
   o.g_plane = xr * o.piece;
   o.g = c.take<u16>((size_t)planes * xr * o.piece);
-  o.dx_split = split_of((long)obman_cdiv(ld, BI) * obman_cdiv(p.rows, BJ), o.piece);
-  o.dw_split = split_of((long)obman_cdiv(ld, BI) * obman_cdiv(o.piece, BJ), xr);
-  o.dx_slabs = c.take<float>(need_x ? (size_t)o.dx_split * p.rows * ld : 0);
-  o.dw_slabs = c.take<float>(need_w ? (size_t)o.dw_split * o.piece * ld : 0);
+  o.parts = parts_of(need_x ? (long)obman_cdiv(ld, BI) * obman_cdiv(p.rows, BJ) : 0, o.piece * terms, need_w ? (long)obman_cdiv(ld, BI) * obman_cdiv(o.piece, BJ) : 0, xr * terms);
+  o.dx_slabs = c.take<float>(need_x ? (size_t)o.parts.x * p.rows * ld : 0);
+  o.dw_slabs = c.take<float>(need_w ? (size_t)o.parts.w * o.piece * ld : 0);
   o.sums = c.take<float>(need_b ? (size_t)(xr / BJ) * o.piece : 0);
   o.bytes = c.at;
   return o;
@@ -847,16 +1083,14 @@ static int blocks_for(long items) {
   return (int)(b < 1 ? 1 : b > 8192 ? 8192 : b);
 }
 
-template <bool A_KR, bool B_KR, class Epi, int T, int TERMS>
-static int launch_gemm(const Gemm& g, int splits, const Epi& epi, hipStream_t st) {
-  static std::atomic<unsigned> done{0};
-  const int dev = current_device();
-  if (!(done.load(std::memory_order_relaxed) >> dev & 1)) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_kernel<A_KR, B_KR, T, TERMS, Epi>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES);
-    if (e != hipSuccess) return (int)e;
-    done.fetch_or(1u << dev, std::memory_order_relaxed);
-  }
-  gemm_kernel<A_KR, B_KR, T, TERMS, Epi><<<dim3(g.ti * g.tj, splits), 256, LDS_BYTES, st>>>(g, epi);
+static Gemm gemm_of(const Side& a, const Side& b, long ni, long nj, long k, int parts, int na, int nb) {
+  return Gemm{a, b, ni, nj, k, up((k + parts - 1) / parts, BK), obman_cdiv(ni, BI), obman_cdiv(nj, BJ), parts, na, nb};
+}
+template <int T, int TERMS, class Epi>
+static int launch_logits(const Gemm& g, const Epi& epi, hipStream_t st) {
+  const hipError_t a = allow_lds<logits_kernel<T, TERMS, Epi>, LDS_BYTES>();
+  if (a != hipSuccess) return (int)a;
+  logits_kernel<T, TERMS, Epi><<<g.ti * g.tj, WAVES * 64, LDS_BYTES, st>>>(g, epi);
   OBMAN_LAUNCH_CHECK();
   return 0;
 }
@@ -878,116 +1112,129 @@ static int operands(const obman_class_loss_params& p, const Keep& k, float* max_
 }
 
 static int check(const obman_class_loss_params* p) {
-  if (!p || !p->x || !p->w || !p->target) return -1;
+  if (!p || !p->target) return -1;
   if (p->rows <= 0 || p->classes <= 0 || p->width <= 0 || p->width > 16384) return -2;
   if (p->rows > MOST_ROWS || p->classes > MOST_ROWS) return -2;
   if (p->type < 0 || p->type > 2 || p->reduction < 0 || p->reduction > 2) return -3;
   return 0;
 }
 
+// |g| in 16 bits: scaled in fp16
+static float g_scale_of(int type) { return type == BF16 ? 1.f : G_SCALE; }
+
 template <int T, int TERMS>
 static int forward(const obman_class_loss_params& p, const Keep& k, const Forward& o, hipStream_t st) {
   constexpr bool split = TERMS == 3;
-  const long kk = k.blocks * 32;
-  const Gemm g{k.w, k.x, p.classes, p.rows, kk, kk, o.ti, obman_cdiv(p.rows, BJ), 0, 0};
   const Stats<split> epi{{Scale{split ? k.scales : nullptr, split ? k.scales + 1 : nullptr}, p.bias, p.type, 0, p.classes}, p.target, p.target_wide, o.part, o.picked};
-  return launch_gemm<false, false, Stats<split>, T, TERMS>(g, 1, epi, st);
+  return launch_logits<T, TERMS>(gemm_of(k.w, k.x, p.classes, p.rows, k.blocks * 32, 1, 0, 0), epi, st);
 }
 
 template <int T, int TERMS>
-static int backward(const obman_class_loss_params& p, const Keep& k, const Backward& o, void* dx, void* dw, void* db, hipStream_t st) {
+static int backward(const obman_class_loss_params& p, const Keep& k, const Backward& o, const RowConst* rows, const Alpha& alpha, void* dx, void* dw, void* db, hipStream_t st) {
   constexpr bool split = TERMS == 3;
   const float *sx = split ? k.scales : nullptr, *sw = split ? k.scales + 1 : nullptr;
   const long xr = k.x.rows;
   const int ld = k.blocks * 32, size = p.type == F32 ? 4 : 2;
-  int e;
+  const hipError_t a = allow_lds<grads_kernel<T, TERMS>, LDS_BYTES>();
+  if (a != hipSuccess) return (int)a;
   for (long v0 = 0; v0 < p.classes; v0 += o.piece) {
     const long nv = p.classes - v0 < o.piece ? p.classes - v0 : o.piece, kv = up(nv, 32);
+    const bool last = v0 + nv == p.classes;
     const Side w{k.wp + v0 * 32, k.w.plane, k.w.rows}, gs{o.g, o.g_plane, xr};
-    const Gemm gg{w, k.x, kv, p.rows, ld, ld, obman_cdiv(kv, BI), (int)(xr / BJ), 0, 0};
-    const Grad<T, split> ge{{Scale{sx, sw}, p.bias, p.type, v0, v0 + nv}, o.rows, xr, o.g, o.g_plane, (int)kv, db ? o.sums : nullptr};
-    if ((e = launch_gemm<false, false, Grad<T, split>, T, TERMS>(gg, 1, ge, st))) return e;
-    if (dx) {
-      const Gemm gx{w, gs, ld, p.rows, kv, split_len(kv, o.dx_split), obman_cdiv(ld, BI), obman_cdiv(p.rows, BJ), k.blocks, 0};
-      const Slab ex{o.dx_slabs, p.rows * ld, ld, v0 > 0};
-      if ((e = launch_gemm<true, false, Slab, T, TERMS>(gx, o.dx_split, ex, st))) return e;
-    }
-    if (dw) {
-      const Gemm gw{k.x, gs, ld, nv, xr, split_len(xr, o.dw_split), obman_cdiv(ld, BI), obman_cdiv(nv, BJ), k.blocks, (int)(kv / 32)};
-      const Slab ew{o.dw_slabs, o.piece * ld, ld, 0};
-      if ((e = launch_gemm<true, true, Slab, T, TERMS>(gw, o.dw_split, ew, st))) return e;
-      finish_kernel<<<blocks_for(nv * (p.width / 4 + 1)), 256, 0, st>>>(o.dw_slabs, o.dw_split, o.piece * ld, nv, ld, p.width, o.alpha, sx,
-                                                                        static_cast<char*>(dw) + (size_t)v0 * p.width * size, p.type);
+    const Grad<T, split> ge{{Scale{sx, sw}, p.bias, p.type, v0, v0 + nv}, rows, p.rows, xr, o.g, o.g_plane, (int)kv, db ? o.sums : nullptr};
+    if (const int e = launch_logits<T, TERMS>(gemm_of(w, k.x, kv, xr, ld, 1, 0, 0), ge, st)) return e;
+    const Gemm gx = gemm_of(w, gs, ld, p.rows, kv, o.parts.x, k.blocks, 0), gw = gemm_of(k.x, gs, ld, nv, xr, o.parts.w, k.blocks, (int)(kv / 32));
+    const int nx = dx ? gx.ti * gx.tj * gx.parts : 0, nw = dw ? gw.ti * gw.tj * gw.parts : 0;
+    if (nx + nw) {
+      const int second = o.parts.x_first ? nw : nx, first = nx + nw - second;
+      grads_kernel<T, TERMS><<<((first + 7) & ~7) + second, WAVES * 64, LDS_BYTES, st>>>(gx, Slab{o.dx_slabs, p.rows * ld, ld, v0 > 0}, nx, gw,
+                                                                                         Slab{o.dw_slabs, o.piece * ld, ld, 0}, nw, o.parts.x_first);
       OBMAN_LAUNCH_CHECK();
     }
-    if (db) {
-      bias_kernel<<<obman_cdiv(nv, 256), 256, 0, st>>>(o.sums, (int)(xr / BJ), (int)kv, nv, o.alpha, static_cast<char*>(db) + (size_t)v0 * size, p.type);
+    const Finish fx{o.dx_slabs, o.parts.x, p.rows * ld, dx && last ? p.rows : 0, sw, dx};
+    const Finish fw{o.dw_slabs, o.parts.w, o.piece * ld, dw ? nv : 0, sx, static_cast<char*>(dw) + (size_t)v0 * p.width * size};
+    const FinishBias fb{o.sums, (int)(xr / BJ), (int)kv, db ? nv : 0, static_cast<char*>(db) + (size_t)v0 * size};
+    const long most = (fx.rows > fw.rows ? fx.rows : fw.rows) * ((p.width + 3) / 4);
+    if (most || db) {
+      finish_kernel<<<dim3(blocks_for(most > fb.classes ? most : fb.classes), db ? 3 : 2), 256, 0, st>>>(fx, fw, fb, ld, p.width, alpha, p.type);
       OBMAN_LAUNCH_CHECK();
     }
-  }
-  if (dx) {
-    finish_kernel<<<blocks_for(p.rows * (p.width / 4 + 1)), 256, 0, st>>>(o.dx_slabs, o.dx_split, p.rows * ld, p.rows, ld, p.width, o.alpha, sw, dx, p.type);
-    OBMAN_LAUNCH_CHECK();
   }
   return 0;
 }
+
+constexpr long WHOLE_PARTS = 16384;  // tile statistics that one block joins: a second launch costs more than the idle CUs
 
 }  // namespace cl
 
 extern "C" {
 
-long obman_class_loss_keep_bytes(const obman_class_loss_params* p) {
+int obman_class_loss_sizes(const obman_class_loss_params* p, int keeps, int need_x, int need_w, int need_b, long* keep_bytes, long* fwd_bytes, long* bwd_bytes) {
   const int e = cl::check(p);
-  return e ? e : (long)cl::keep_of(*p, nullptr).bytes;
+  if (e) return e;
+  if (!keep_bytes || !fwd_bytes || !bwd_bytes) return -1;
+  const cl::Keep k = cl::keep_of(*p, nullptr);
+  cl::Few few;
+  *keep_bytes = (long)k.bytes;
+  *fwd_bytes = !keeps && cl::few_of(*p, nullptr, &few) ? (long)few.bytes : (long)(cl::forward_of(*p, nullptr).bytes + (keeps ? 0 : k.bytes));
+  *bwd_bytes = (long)cl::backward_of(*p, k, nullptr, need_x, need_w, need_b).bytes;
+  return 0;
 }
 
-long obman_class_loss_fwd_ws_bytes(const obman_class_loss_params* p) {
-  const int e = cl::check(p);
-  return e ? e : (long)cl::forward_of(*p, nullptr).bytes;
-}
-
-int obman_class_loss_fwd(const obman_class_loss_params* p, void* keep, void* ws, float* loss, float* lse, float* norm, obman_stream_t stream) {
+int obman_class_loss_fwd(const obman_class_loss_params* p, void* keep, void* ws, float* loss, obman_stream_t stream) {
   int e = cl::check(p);
   if (e) return e;
-  if (!keep || !ws || !loss || !lse || !norm) return -1;
+  if (!p->x || !p->w || !ws || !loss) return -1;
   hipStream_t st = (hipStream_t)stream;
-  const cl::Keep k = cl::keep_of(*p, keep);
+  cl::Few few;
+  if (!keep && cl::few_of(*p, ws, &few))
+    return p->type == cl::F32    ? cl::few<cl::F32>(*p, few, loss, st)
+           : p->type == cl::BF16 ? cl::few<cl::BF16>(*p, few, loss, st)
+                                 : cl::few<cl::F16>(*p, few, loss, st);
+  const cl::Keep k = cl::keep_of(*p, keep ? keep : static_cast<char*>(ws) + cl::forward_of(*p, nullptr).bytes);
   const cl::Forward o = cl::forward_of(*p, ws);
   if ((e = cl::operands(*p, k, o.max_part, st))) return e;
   e = p->type == cl::F32    ? cl::forward<cl::F16, 3>(*p, k, o, st)
       : p->type == cl::BF16 ? cl::forward<cl::BF16, 1>(*p, k, o, st)
                             : cl::forward<cl::F16, 1>(*p, k, o, st);
   if (e) return e;
-  cl::join_rows_kernel<<<o.row_blocks, 256, 0, st>>>(o.part, o.ti, p->rows, p->classes, o.picked, p->target, p->target_wide, p->ignore_index, lse,
-                                                     p->reduction ? nullptr : loss, p->reduction ? o.sums : nullptr);
+  cl::RowConst* consts = keep && p->reduction ? k.rows : nullptr;
+  const float gs = cl::g_scale_of(p->type);
+  if (p->rows * o.ti <= cl::WHOLE_PARTS) {
+    cl::join_rows_kernel<true><<<1, 1024, 0, st>>>(o.part, o.ti, p->rows, p->classes, o.picked, p->target, p->target_wide, p->ignore_index, p->reduction, gs, k.lse, loss,
+                                                   consts, nullptr, k.norm);
+    OBMAN_LAUNCH_CHECK();
+    return 0;
+  }
+  cl::join_rows_kernel<false><<<o.row_blocks, 256, 0, st>>>(o.part, o.ti, p->rows, p->classes, o.picked, p->target, p->target_wide, p->ignore_index, p->reduction, gs, k.lse,
+                                                            loss, consts, o.sums, nullptr);
   OBMAN_LAUNCH_CHECK();
   if (p->reduction) {
-    cl::reduce_kernel<<<1, 256, 0, st>>>(o.sums, o.row_blocks, p->reduction == 2, loss, norm);
+    cl::reduce_kernel<<<1, 256, 0, st>>>(o.sums, o.row_blocks, p->reduction == 2, loss, k.norm);
     OBMAN_LAUNCH_CHECK();
   }
   return 0;
 }
 
-long obman_class_loss_bwd_ws_bytes(const obman_class_loss_params* p, int need_x, int need_w, int need_b) {
+int obman_class_loss_bwd(const obman_class_loss_params* p, const void* keep, const float* g_loss, void* ws, void* dx, void* dw, void* db, obman_stream_t stream) {
   const int e = cl::check(p);
-  return e ? e : (long)cl::backward_of(*p, cl::keep_of(*p, nullptr), nullptr, need_x, need_w, need_b).bytes;
-}
-
-int obman_class_loss_bwd(const obman_class_loss_params* p, const void* keep, const float* lse, const float* norm, const float* g_loss, void* ws, void* dx, void* dw,
-                         void* db, obman_stream_t stream) {
-  int e = cl::check(p);
   if (e) return e;
-  if (!keep || !ws || !lse || !g_loss || (p->reduction && !norm)) return -1;
+  if (!keep || !ws || !g_loss) return -1;
   if (!dx && !dw && !db) return 0;
   hipStream_t st = (hipStream_t)stream;
   const cl::Keep k = cl::keep_of(*p, const_cast<void*>(keep));
   const cl::Backward o = cl::backward_of(*p, k, ws, dx != nullptr, dw != nullptr, db != nullptr);
-  cl::rows_kernel<<<obman_cdiv(p->rows, 1024), 1024, 0, st>>>(lse, p->target, p->target_wide, p->ignore_index, p->rows, g_loss, p->reduction == 0, norm,
-                                                              p->type == cl::BF16 ? 1.f : cl::G_SCALE, o.rows, o.alpha);
-  OBMAN_LAUNCH_CHECK();
-  return p->type == cl::F32    ? cl::backward<cl::F16, 3>(*p, k, o, dx, dw, db, st)
-         : p->type == cl::BF16 ? cl::backward<cl::BF16, 1>(*p, k, o, dx, dw, db, st)
-                               : cl::backward<cl::F16, 1>(*p, k, o, dx, dw, db, st);
+  const float gs = cl::g_scale_of(p->type);
+  cl::Alpha alpha{g_loss, k.norm, 1.f / gs};
+  if (!p->reduction) {
+    cl::rows_kernel<<<obman_cdiv(p->rows, 1024), 1024, 0, st>>>(k.lse, p->target, p->target_wide, p->ignore_index, p->rows, g_loss, gs, o.rows, o.alpha);
+    OBMAN_LAUNCH_CHECK();
+    alpha = cl::Alpha{o.alpha, nullptr, 1.f / gs};
+  }
+  const cl::RowConst* rows = p->reduction ? k.rows : o.rows;
+  return p->type == cl::F32    ? cl::backward<cl::F16, 3>(*p, k, o, rows, alpha, dx, dw, db, st)
+         : p->type == cl::BF16 ? cl::backward<cl::BF16, 1>(*p, k, o, rows, alpha, dx, dw, db, st)
+                               : cl::backward<cl::F16, 1>(*p, k, o, rows, alpha, dx, dw, db, st);
 }
 
 }  // extern "C"

@@ -922,55 +922,73 @@ _CLASS_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
+class _on_device:
+    """The launches of the block go to the tensors' device, on its current stream (``torch.cuda.device`` without its 3 us where the
+    device is the current one already)."""
+
+    def __init__(self, device):
+        self.ctx = None
+        if _RAW_DEVICE is None or _RAW_DEVICE() != device.index:
+            self.ctx = torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
 def _class_loss_params(x, weight, bias, target, ignore_index, reduction):
-    p = _lib.ClassLossParams()
-    p.x, p.w, p.bias, p.target = x.data_ptr(), weight.data_ptr(), _ptr(bias), target.data_ptr()
-    p.rows, p.classes, p.ignore_index = target.numel(), weight.shape[0], ignore_index
-    p.width, p.type, p.target_wide, p.reduction = weight.shape[1], _CLASS_TYPES[weight.dtype], int(target.dtype == torch.int64), reduction
-    return p
+    return _lib.ClassLossParams(x.data_ptr(), weight.data_ptr(), _ptr(bias), target.data_ptr(), target.numel(), weight.shape[0], ignore_index,
+                                weight.shape[1], _CLASS_TYPES[weight.dtype], target.dtype == torch.int64, reduction)
 
 
-def _class_loss_ws(nbytes, what, device):
-    if nbytes < 0:
-        _lib.check(int(nbytes), what)
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)  # of this call alone: recorded into a graph it is the graph's
+_SIZES = _ct.c_long * 3
+
+
+def _class_loss_forward(x, weight, bias, target, ignore_index, reduction, keeps):
+    """-> loss, and with ``keeps`` what the backward pass needs.  All scratch is of this call alone: recorded into a graph it is the graph's."""
+    dev, lib = x.device, _lib.lib()
+    p = _class_loss_params(x, weight, bias, target, ignore_index, reduction)
+    at, n = _ct.addressof(p), _SIZES()
+    to = _ct.addressof(n)
+    _lib.check(lib.obman_class_loss_sizes(at, int(keeps), 0, 0, 0, to, to + 8, to + 16), "obman_class_loss_sizes")
+    loss = torch.empty(target.shape if reduction == 0 else (), dtype=torch.float32, device=dev)
+    keep = torch.empty(n[0], dtype=torch.uint8, device=dev) if keeps else None
+    ws = torch.empty(n[1], dtype=torch.uint8, device=dev)
+    with _on_device(dev):
+        _lib.check(lib.obman_class_loss_fwd(at, _ptr(keep), ws.data_ptr(), loss.data_ptr(), _stream()), "obman_class_loss_fwd")
+    return loss, keep
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, target, ignore_index, reduction):
-        x, weight, target = x.contiguous(), weight.contiguous(), target.contiguous()
-        bias = None if bias is None else bias.contiguous()
-        rows, o = target.numel(), dict(dtype=torch.float32, device=x.device)
-        loss = torch.empty(target.shape if reduction == 0 else (), **o)
-        lse, norm = torch.empty(rows, **o), torch.empty((), **o)
-        lib = _lib.lib()
-        p = _class_loss_params(x, weight, bias, target, ignore_index, reduction)
-        with torch.cuda.device(x.device):
-            keep = _class_loss_ws(lib.obman_class_loss_keep_bytes(_ct.addressof(p)), "obman_class_loss_keep_bytes", x.device)
-            ws = _class_loss_ws(lib.obman_class_loss_fwd_ws_bytes(_ct.addressof(p)), "obman_class_loss_fwd_ws_bytes", x.device)
-            _lib.check(lib.obman_class_loss_fwd(_ct.addressof(p), keep.data_ptr(), ws.data_ptr(), loss.data_ptr(), lse.data_ptr(), norm.data_ptr(), _stream()),
-                       "obman_class_loss_fwd")
-        ctx.save_for_backward(x, weight, bias, target, keep, lse, norm)
+        loss, keep = _class_loss_forward(x, weight, bias, target, ignore_index, reduction, True)
+        ctx.save_for_backward(x, weight, bias, target, keep)
         ctx.cfg = (ignore_index, reduction)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss):
-        x, weight, bias, target, keep, lse, norm = ctx.saved_tensors
+        x, weight, bias, target, keep = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         g_loss = _dev(g_loss, "grad")
+        dev, lib = x.device, _lib.lib()
         dx = torch.empty_like(x) if need_x else None
         dw = torch.empty_like(weight) if need_w else None
         db = torch.empty_like(bias) if need_b else None
-        lib = _lib.lib()
         p = _class_loss_params(x, weight, bias, target, *ctx.cfg)
-        with torch.cuda.device(x.device):
-            ws = _class_loss_ws(lib.obman_class_loss_bwd_ws_bytes(_ct.addressof(p), int(need_x), int(need_w), int(need_b)),
-                                "obman_class_loss_bwd_ws_bytes", x.device)
-            _lib.check(lib.obman_class_loss_bwd(_ct.addressof(p), keep.data_ptr(), lse.data_ptr(), norm.data_ptr(), g_loss.data_ptr(), ws.data_ptr(), _ptr(dx),
-                                                _ptr(dw), _ptr(db), _stream()), "obman_class_loss_bwd")
+        at, n = _ct.addressof(p), _SIZES()
+        to = _ct.addressof(n)
+        _lib.check(lib.obman_class_loss_sizes(at, 1, need_x, need_w, need_b, to, to + 8, to + 16), "obman_class_loss_sizes")
+        ws = torch.empty(n[2], dtype=torch.uint8, device=dev)
+        with _on_device(dev):
+            _lib.check(lib.obman_class_loss_bwd(at, keep.data_ptr(), g_loss.data_ptr(), ws.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), _stream()),
+                       "obman_class_loss_bwd")
         return dx, dw, db, None, None, None
 
 
@@ -1007,4 +1025,8 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
     if target.numel() == 0:  # no rows: nothing to launch; the graph stays connected
         zero = x.float().sum() * 0.0
         return x.float().sum(-1) if reduction == "none" else zero
-    return _LinearCrossEntropy.apply(x, weight, bias, target, int(ignore_index), _REDUCTIONS[reduction])
+    x, weight, target = x.contiguous(), weight.contiguous(), target.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return _LinearCrossEntropy.apply(x, weight, bias, target, int(ignore_index), _REDUCTIONS[reduction])
+    return _class_loss_forward(x, weight, bias, target, int(ignore_index), _REDUCTIONS[reduction], False)[0]
