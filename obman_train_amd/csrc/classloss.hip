@@ -38,29 +38,33 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 enum { F32 = 0, BF16 = 1, F16 = 2 };
 
-// Operands are kept in blocks of 32 columns, [columns / 32][rows][32]: whatever a step of 32 needs of one - 32 columns of 256 rows, or
-// 32 rows of 8 blocks - is read in runs of 1 KB or more.  (Row-major, a step reads 64 of each row's bytes, half cache lines: the path
-// from L2 to LDS then holds the products at 900 Tflop/s; without any such reads they run at 1170 - 1270.)  Rows are padded with zeros
-// to whole tiles, so no address leaves an operand.
+// Operands are kept in blocks of columns, [blocks][rows][64 bytes]: 32 columns of a 16-bit operand, or 16 of a split one, hi beside lo.
+// Whatever a step of the contraction needs of one - a block of 256 rows, or some rows of all blocks - is read in runs of 1 KB or more.
+// (Row-major, a step reads 64 of each row's bytes, half cache lines, and the path from L2 to LDS is what holds the products back:
+// without those reads they run at 1170 - 1270 Tflop/s.)  A split step of 16 has its two planes loaded once for three products.  Rows
+// are padded with zeros to whole tiles, so no address leaves an operand.
 // Tile 256 x 128, four waves of 128 x 64.  72 KB of LDS, so two blocks share a CU and one's epilogue and waits run under the other's
 // products.  (256 x 256 with eight waves, four steps deep, one block on a CU, fetches a third less; at 19 200 x 64 050 x 512 it
 // measured 1 474 us for the forward product against 1 330, 328 against 304 for g, 290 against 300 and 250 against 253 for the other two.)
-constexpr int BI = 256, BJ = 128, BK = 32, WAVES = 4, STAGES = 3;
-constexpr int A_BYTES = BI * BK * 2, STAGE_BYTES = A_BYTES + BJ * BK * 2;
+constexpr int BI = 256, BJ = 128, WAVES = 4, STAGES = 3;
+constexpr int A_BYTES = BI * 64, STAGE_BYTES = A_BYTES + BJ * 64;
 constexpr int BIAS_AT = STAGES * STAGE_BYTES, LDS_BYTES = BIAS_AT + BI * 4;
 constexpr int SLOTS = 512;  // blocks that run at a time
-constexpr long MOST_ROWS = 1L << 22;         // of an operand: eight blocks of its columns stay within 32-bit offsets
+constexpr long MOST_ROWS = 1L << 22;  // of an operand: sixteen blocks of its columns stay within 32-bit offsets
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float G_SCALE = 16384.f;  // |g| / max|c| <= 1 in fp16
 
-struct Side {       // [planes][blocks][rows][32]
+template <bool SPLIT>
+constexpr int Step = SPLIT ? 16 : 32;  // columns of a block, and the contraction of a step
+
+struct Side {  // [blocks][rows][32]
   const u16* p;
-  long plane, rows; // elements from the hi to the lo plane; rows of a block
+  long rows;   // of a block
 };
 struct Gemm {
   Side a, b;
   long ni, nj;      // extents of the result
-  long k;           // contraction, a multiple of 32
+  long k;           // contraction, a multiple of the step
   long k_part;      // of it per part
   int ti, tj, parts; // tiles, and parts of the contraction
   int na, nb;       // column blocks of a / b (an operand whose rows are contracted: tiles that run over its columns repeat the last block)
@@ -71,53 +75,59 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, unsigned lds, un
   asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(r) : "memory", "m0");
 }
 
-// One operand's tile, R (i or j) x 32 k, 64-byte rows in LDS.  KC: the rows are i or j and the 32 columns are k; 16-byte chunks are placed at
-// chunk ^ (row >> 2 & 3), so that the wide reads do not meet in a bank (the DMA writes LDS linearly: the source address carries the
-// swizzle).  KR: the rows are k, 32 of them for each of R / 32 column blocks, read by the transposing LDS reads, which take four
-// whole rows at a time and need no swizzle.
-template <bool KR, int R>
+// One operand's tile for a step of Step<SPLIT> k, R (i or j) wide, in 64-byte rows of LDS.  KC: the rows are i or j and their columns
+// are k; 16-byte chunks are placed at chunk ^ (row >> 2 & 3), so that the wide reads do not meet in a bank (the DMA writes LDS
+// linearly: the source address carries the swizzle).  KR: the rows are k, a step of them for each column block, read by the
+// transposing LDS reads, which take four whole rows at a time; with split operands they take half of each, and every other block
+// has its halves exchanged.
+template <bool KR, int R, bool SPLIT>
 struct Operand {
-  static constexpr int N = R * BK * 2 / 1024 / WAVES;  // wave-wide loads of 1 KB per wave and step
+  static constexpr int N = R * 64 / 1024 / WAVES;  // wave-wide loads of 1 KB per wave and step
   const u16* base;  // at the next step's k
   long step;
   unsigned voff[N];
   __device__ __forceinline__ void init(const Side& s, int first_block, int blocks, int wave, int lane) {
-    step = KR ? BK * 32 : s.rows * 32;
+    step = KR ? Step<SPLIT> * 32 : s.rows * 32;
+    const int last = blocks - 1 - first_block;
 #pragma unroll
     for (int q = 0; q < N; ++q) {
       const int at = wave * N + q;
       if constexpr (!KR) {
         voff[q] = at * 1024 + (lane >> 2) * 64 + ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
+      } else if constexpr (!SPLIT) {
+        const int b = at >> 1;
+        voff[q] = (unsigned)((b < last ? b : last) * s.rows * 64) + (at & 1) * 1024 + lane * 16;
       } else {
-        const int last = blocks - 1 - first_block, b = at >> 1;
-        voff[q] = (unsigned)((b < last ? b : last) * s.rows * 64 + (at & 1) * 1024 + lane * 16);
+        voff[q] = (unsigned)((at < last ? at : last) * s.rows * 64) + (lane >> 2) * 64 + ((lane & 3) ^ ((at & 1) << 1)) * 16;
       }
     }
   }
-  // row0: first row (KC: of the tile; KR: of the contraction), k0: first column of the contraction (KC) or of the tile (KR)
-  __device__ __forceinline__ void start(const Side& s, int pl, long row0, long col0) { base = s.p + (pl ? s.plane : 0) + (col0 * s.rows + row0 * 32); }
+  // row0: first row (KC: of the tile; KR: of the contraction), col0: first column of the contraction (KC) or of the tile (KR)
+  __device__ __forceinline__ void start(const Side& s, long row0, long col0) { base = s.p + (col0 / Step<SPLIT> * s.rows + row0) * 32; }
   __device__ __forceinline__ void issue(unsigned lds, int wave) {
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<u16*>(base), 0, 0x7ffffff0, 0x00020000);
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<u16*>(base), 0, (int)0xfffffff0u, 0x00020000);
 #pragma unroll
     for (int q = 0; q < N; ++q) dma16(r, lds + wave * (N * 1024) + q * 1024, voff[q]);
     base += step;
   }
 };
 
-// fragment of 32 rows x 16 k: lane -> row lane % 32, k = 8 (lane / 32) .. + 7
-template <bool KR>
+// fragment of 32 rows x 16 k: lane -> row lane % 32, k = 8 (lane / 32) .. + 7; of the step's two halves, or of hi and lo
+template <bool KR, bool SPLIT>
 struct Frag {
   unsigned off[2];
   __device__ __forceinline__ void init(int first_row, int lane) {  // first_row: a multiple of 32
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      if constexpr (!KR) off[ks] = (first_row + (lane & 31)) * 64 + ((2 * ks + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16;
+    for (int h = 0; h < 2; ++h) {
       // the transposing read: in a group of 16 lanes, lane c receives element c of the four rows that lanes 4 r .. 4 r + 3 point at
-      else off[ks] = first_row * 64 + (ks * 16 + 8 * (lane >> 5) + ((lane & 15) >> 2)) * 64 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+      const int k = 8 * (lane >> 5) + ((lane & 15) >> 2), right = (lane >> 4) & 1;
+      if constexpr (!KR) off[h] = (first_row + (lane & 31)) * 64 + ((2 * h + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16;
+      else if constexpr (!SPLIT) off[h] = first_row * 64 + (h * 16 + k) * 64 + right * 32 + (lane & 3) * 8;
+      else off[h] = first_row * 64 + right * 1024 + k * 64 + (h ^ right) * 32 + (lane & 3) * 8;
     }
   }
-  __device__ __forceinline__ u32x4 read(const char* tile, int f, int ks) const {
-    const char* p = tile + off[ks] + f * 2048;
+  __device__ __forceinline__ u32x4 read(const char* tile, int f, int h) const {
+    const char* p = tile + off[h] + f * 2048;
     if constexpr (!KR) return *reinterpret_cast<const u32x4*>(p);
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p));
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p + 4 * 64));
@@ -320,7 +330,6 @@ struct Grad {
   const RowConst* rows;
   long n_rows, rows_padded;
   u16* out;
-  long plane;
   int columns;      // of out
   float* sums;      // [tj][columns]: the bias gradient's parts, summed before g is rounded
   __device__ __forceinline__ void before(const Gemm&, const Ctx& c, f32x16 (&acc)[4][2]) const { bias.before(c, acc); }
@@ -350,7 +359,7 @@ struct Grad {
           for (int q = 0; q < 16; ++q) acc[fi][fj][q] *= sign;
       }
       // lanes l and l + 32 hold classes 0 .. 3 and 4 .. 7 of each 8: an exchange gives each 8 in a row, 16 bytes
-      u16* o = out + ((c.i0 + c.wi * 128) * rows_padded + r * 32) + 8 * (c.lane >> 5);
+      u16* o = out + ((c.i0 + c.wi * 128) / Step<SPLIT> * rows_padded + r) * 32 + 8 * (c.lane >> 5);
 #pragma unroll
       for (int fi = 0; fi < 4; ++fi) {
         if (c.i0 + c.wi * 128 + fi * 32 >= columns) continue;
@@ -366,7 +375,7 @@ struct Grad {
               hi[u][e] = hx | (unsigned)hy << 16;
               if constexpr (SPLIT) lo[u][e] = narrow<T>(x - widen<T>(hx)) | (unsigned)narrow<T>(y - widen<T>(hy)) << 16;
             }
-          u16* to = o + fi * 32 * rows_padded + q * 8;
+          u16* to = o + (SPLIT ? (fi * 2 + q / 2) * rows_padded * 32 : fi * rows_padded * 32 + q * 8);
           {
             const u32x2 s0 = __builtin_amdgcn_permlane32_swap(hi[0][0], hi[1][0], false, false);
             const u32x2 s1 = __builtin_amdgcn_permlane32_swap(hi[0][1], hi[1][1], false, false);
@@ -375,7 +384,7 @@ struct Grad {
           if constexpr (SPLIT) {
             const u32x2 s0 = __builtin_amdgcn_permlane32_swap(lo[0][0], lo[1][0], false, false);
             const u32x2 s1 = __builtin_amdgcn_permlane32_swap(lo[0][1], lo[1][1], false, false);
-            *reinterpret_cast<u32x4*>(to + plane) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+            *reinterpret_cast<u32x4*>(to + 16) = u32x4{s0[0], s1[0], s0[1], s1[1]};
           }
         }
       }
@@ -430,8 +439,8 @@ struct Slab {
   }
 };
 
-// C[i, j] = sum_k A(i, k) B(j, k); TERMS = 3: both operands in two planes
-template <bool A_KR, bool B_KR, int T, int TERMS, class Epi>
+// C[i, j] = sum_k A(i, k) B(j, k)
+template <bool A_KR, bool B_KR, int T, bool SPLIT, class Epi>
 __device__ __forceinline__ void gemm(const Gemm& g, const Epi& epi, int id, char* smem) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int bi, bj, part;
@@ -440,46 +449,30 @@ __device__ __forceinline__ void gemm(const Gemm& g, const Epi& epi, int id, char
   bj = __builtin_amdgcn_readfirstlane(bj);
   part = __builtin_amdgcn_readfirstlane(part);
   const Ctx ctx{(long)bi * BI, (long)bj * BJ, wave & 1, wave >> 1, lane, tid, bi, bj, part, smem, smem + BIAS_AT};
-  Operand<A_KR, BI> oa;
-  Operand<B_KR, BJ> ob;
-  oa.init(g.a, bi * (BI / 32), g.na, wave, lane);
-  ob.init(g.b, bj * (BJ / 32), g.nb, wave, lane);
-  Frag<A_KR> fa;
-  Frag<B_KR> fb;
+  constexpr int K = Step<SPLIT>;
+  Operand<A_KR, BI, SPLIT> oa;
+  Operand<B_KR, BJ, SPLIT> ob;
+  oa.init(g.a, bi * (BI / K), g.na, wave, lane);
+  ob.init(g.b, bj * (BJ / K), g.nb, wave, lane);
+  Frag<A_KR, SPLIT> fa;
+  Frag<B_KR, SPLIT> fb;
   fa.init(ctx.wi * 128, lane);
   fb.init(ctx.wj * 64, lane);
   const long kb = part * g.k_part, ke = kb + g.k_part < g.k ? kb + g.k_part : g.k;
-  const int steps = ke > kb ? (int)((ke - kb) / BK) * TERMS : 0;
+  const int steps = ke > kb ? (int)((ke - kb) / K) : 0;
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
 
   f32x16 acc[4][2];
   epi.before(g, ctx, acc);
-  int term = TERMS == 3 ? 0 : 2, left = (int)((ke - kb) / BK);  // terms: lo hi, hi lo, hi hi
-  const int per_term = left;
-  const auto start = [&]() {
-    oa.start(g.a, term == 0, A_KR ? kb : ctx.i0, A_KR ? ctx.i0 : kb);
-    ob.start(g.b, term == 1, B_KR ? kb : ctx.j0, B_KR ? ctx.j0 : kb);
-  };
-  start();
+  oa.start(g.a, A_KR ? kb : ctx.i0, A_KR ? ctx.i0 : kb);
+  ob.start(g.b, B_KR ? kb : ctx.j0, B_KR ? ctx.j0 : kb);
   unsigned to = lds0;
   const auto issue = [&]() {
     oa.issue(to, wave);
     ob.issue(to + A_BYTES, wave);
     to = to == lds0 + (STAGES - 1) * STAGE_BYTES ? lds0 : to + STAGE_BYTES;
-    if (TERMS == 3 && --left == 0) {
-      left = per_term;
-      ++term;
-      start();
-    }
   };
   const char* from = smem;
-  const auto next = [&](const char* p) { return p == smem + (STAGES - 1) * STAGE_BYTES ? smem : p + STAGE_BYTES; };
-  const auto read = [&](const char* p, int ks, u32x4 (&a)[4], u32x4 (&b)[2]) {
-#pragma unroll
-    for (int f = 0; f < 2; ++f) b[f] = fb.read(p + A_BYTES, f, ks);
-#pragma unroll
-    for (int f = 0; f < 4; ++f) a[f] = fa.read(p, f, ks);
-  };
   const auto products = [&](const u32x4 (&a)[4], const u32x4 (&b)[2]) {
     __builtin_amdgcn_sched_barrier(0);  // the reads before go out first
     __builtin_amdgcn_s_setprio(1);
@@ -490,42 +483,53 @@ __device__ __forceinline__ void gemm(const Gemm& g, const Epi& epi, int id, char
     __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
   };
-  static_assert(Operand<A_KR, BI>::N + Operand<B_KR, BJ>::N == 6, "the counted wait below");
-  u32x4 a0[4], b0[2], a1[4], b1[2];
+  static_assert(Operand<A_KR, BI, SPLIT>::N + Operand<B_KR, BJ, SPLIT>::N == 6, "the counted wait below");
   if (steps > 0) issue();
   if (steps > 1) issue();
   for (int s = 0; s < steps; ++s) {
     // step s has arrived for every wave (only step s + 1 may still be under way), and every wave has read step s - 1, whose slot is next
     if (s + 1 < steps) asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    read(from, 0, a0, b0);
-    read(from, 1, a1, b1);
+    u32x4 a[2][4], b[2][2];  // the step's two halves of 16, or hi and lo
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int f = 0; f < 2; ++f) b[h][f] = fb.read(from + A_BYTES, f, h);
+#pragma unroll
+      for (int f = 0; f < 4; ++f) a[h][f] = fa.read(from, f, h);
+    }
     if (s + 2 < steps) issue();
-    from = next(from);
-    products(a0, b0);
-    products(a1, b1);
+    from = from == smem + (STAGES - 1) * STAGE_BYTES ? smem : from + STAGE_BYTES;
+    if constexpr (SPLIT) {
+      products(a[0], b[0]);
+      products(a[0], b[1]);
+      products(a[1], b[0]);
+    } else {
+      products(a[0], b[0]);
+      products(a[1], b[1]);
+    }
   }
   __syncthreads();
   epi.after(g, ctx, acc);
 }
 
-template <int T, int TERMS, class Epi>
+template <int T, bool SPLIT, class Epi>
 __global__ __launch_bounds__(WAVES * 64, 2) void logits_kernel(Gemm g, Epi epi) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  gemm<false, false, T, TERMS>(g, epi, blockIdx.x, smem);
+  gemm<false, false, T, SPLIT>(g, epi, blockIdx.x, smem);
 }
 
 // dx and dw of a piece of the classes in one launch (each may have no blocks): both read the same g, and their blocks fill each
 // other's last round.  The longer ones come first; first: how many blocks that is, rounded up to whole rounds of the XCDs.
-template <int T, int TERMS>
+template <int T, bool SPLIT>
 __global__ __launch_bounds__(WAVES * 64, 2) void grads_kernel(Gemm gx, Slab ex, int nx, Gemm gw, Slab ew, int nw, int x_first) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int first = ((x_first ? nx : nw) + 7) & ~7;
   const bool is_x = ((int)blockIdx.x < first) == (x_first != 0);
   const int id = (int)blockIdx.x < first ? blockIdx.x : blockIdx.x - first;
   if (id >= (is_x ? nx : nw)) return;
-  if (is_x) gemm<true, false, T, TERMS>(gx, ex, id, smem);
-  else gemm<true, true, T, TERMS>(gw, ew, id, smem);
+  if (is_x) gemm<true, false, T, SPLIT>(gx, ex, id, smem);
+  else gemm<true, true, T, SPLIT>(gw, ew, id, smem);
 }
 
 // ------------------------------------------------------------------------------------------------------- operands and rows
@@ -571,9 +575,9 @@ __device__ float scale_of(const float* __restrict__ part) {
   return m > 0.f ? ldexpf(1.f, e) : 1.f;
 }
 
-// x (grid row 0) and w (1) into blocks of 32 columns, [planes][blocks][padded rows][32]: zeros behind the width, behind the last row
-// and for ignored rows
-struct Pack { const void* src; u16* dst; long rows, padded, plane; };
+// x (grid row 0) and w (1) into blocks of columns, [blocks][padded rows][32]: zeros behind the width, behind the last row and for
+// ignored rows
+struct Pack { const void* src; u16* dst; long rows, padded; };
 template <int TYPE>
 __global__ __launch_bounds__(256) void pack_kernel(Pack px, Pack pw, int width, int chunks, const void* target, int wide, long ignore, const float* __restrict__ part,
                                                   float* __restrict__ scale) {
@@ -622,9 +626,10 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack px, Pack pw, int width, 
         }
       }
     }
-    u16* o = p.dst + ((long)(c >> 5) * p.padded + r) * 32 + (c & 31);
+    constexpr int K = Step<TYPE == F32>;
+    u16* o = p.dst + ((long)(c / K) * p.padded + r) * 32 + c % K;
     *reinterpret_cast<u32x4*>(o) = *reinterpret_cast<u32x4*>(hi);
-    if constexpr (TYPE == F32) *reinterpret_cast<u32x4*>(o + p.plane) = *reinterpret_cast<u32x4*>(lo);
+    if constexpr (TYPE == F32) *reinterpret_cast<u32x4*>(o + 16) = *reinterpret_cast<u32x4*>(lo);
   }
 }
 
@@ -938,7 +943,7 @@ struct Keep {
   u16 *xp, *wp;
   float *scales, *lse, *norm;
   RowConst* rows;
-  int blocks;  // of 32 columns
+  int ld;  // the width, up to whole blocks
   size_t bytes;
 };
 static Keep keep_of(const obman_class_loss_params& p, void* mem) {
@@ -946,16 +951,15 @@ static Keep keep_of(const obman_class_loss_params& p, void* mem) {
   Keep k;
   const int planes = p.type == F32 ? 2 : 1;
   const long xr = up(p.rows, BJ), wr = up(p.classes, BI);
-  k.blocks = obman_cdiv(p.width, 32);
-  const long xn = xr * k.blocks * 32, wn = wr * k.blocks * 32;
+  k.ld = (int)up(p.width, 32);
   k.scales = c.take<float>(4);
   k.norm = k.scales + 2;
   k.lse = c.take<float>(p.rows);
   k.rows = c.take<RowConst>(p.reduction ? p.rows : 0);
-  k.xp = c.take<u16>(xn * planes);
-  k.wp = c.take<u16>(wn * planes);
-  k.x = {k.xp, xn, xr};
-  k.w = {k.wp, wn, wr};
+  k.xp = c.take<u16>(xr * k.ld * planes);
+  k.wp = c.take<u16>(wr * k.ld * planes);
+  k.x = {k.xp, xr};
+  k.w = {k.wp, wr};
   k.bytes = c.at;
   return k;
 }
@@ -1037,7 +1041,7 @@ static Parts parts_of(long tiles_x, long k_x, long tiles_w, long k_w) {
     if (x > 1 && k_x / x < 256) break;
     for (int w = 1; w <= (tiles_w ? 32 : 1); ++w) {
       if (w > 1 && k_w / w < 256) break;
-      const double lx = k_x / BK / x + START, lw = k_w / BK / w + START;
+      const double lx = k_x / 32 / x + START, lw = k_w / 32 / w + START;
       const bool first = !tiles_w || (tiles_x && lx >= lw);
       const double nx = (double)tiles_x * x, nw = (double)tiles_w * w, n = first ? nx : nw, l = first ? lx : lw, shorter = tiles_x && tiles_w ? (first ? lw : lx) : l;
       const double rounds = ceil(n / SLOTS) * l, spread = (nx * lx + nw * lw) / SLOTS + 0.5 * shorter;
@@ -1051,7 +1055,7 @@ struct Backward {
   RowConst* rows;
   float* alpha;
   u16* g;
-  long g_plane, piece;
+  long piece;
   float *dx_slabs, *dw_slabs, *sums;
   Parts parts;
   size_t bytes;
@@ -1059,7 +1063,7 @@ struct Backward {
 static Backward backward_of(const obman_class_loss_params& p, const Keep& k, void* mem, bool need_x, bool need_w, bool need_b) {
   Carve c{static_cast<char*>(mem)};
   Backward o;
-  const int planes = p.type == F32 ? 2 : 1, terms = p.type == F32 ? 3 : 1, ld = k.blocks * 32;
+  const int planes = p.type == F32 ? 2 : 1, terms = p.type == F32 ? 3 : 1, ld = k.ld;
   const long xr = k.x.rows, all = up(p.classes, 32);
   o.rows = c.take<RowConst>(p.reduction ? 0 : p.rows);
   o.alpha = c.take<float>(1);
@@ -1068,7 +1072,6 @@ static Backward backward_of(const obman_class_loss_params& p, const Keep& k, voi
   o.piece = all;
   if (most < all) o.piece = up(all / ((all + most - 1) / most) + 1, BI);  // equal pieces
   if (o.piece > all) o.piece = all;
-  o.g_plane = xr * o.piece;
   o.g = c.take<u16>((size_t)planes * xr * o.piece);
   o.parts = parts_of(need_x ? (long)obman_cdiv(ld, BI) * obman_cdiv(p.rows, BJ) : 0, o.piece * terms, need_w ? (long)obman_cdiv(ld, BI) * obman_cdiv(o.piece, BJ) : 0, xr * terms);
   o.dx_slabs = c.take<float>(need_x ? (size_t)o.parts.x * p.rows * ld : 0);
@@ -1084,13 +1087,13 @@ static int blocks_for(long items) {
 }
 
 static Gemm gemm_of(const Side& a, const Side& b, long ni, long nj, long k, int parts, int na, int nb) {
-  return Gemm{a, b, ni, nj, k, up((k + parts - 1) / parts, BK), obman_cdiv(ni, BI), obman_cdiv(nj, BJ), parts, na, nb};
+  return Gemm{a, b, ni, nj, k, up((k + parts - 1) / parts, 32), obman_cdiv(ni, BI), obman_cdiv(nj, BJ), parts, na, nb};
 }
-template <int T, int TERMS, class Epi>
+template <int T, bool SPLIT, class Epi>
 static int launch_logits(const Gemm& g, const Epi& epi, hipStream_t st) {
-  const hipError_t a = allow_lds<logits_kernel<T, TERMS, Epi>, LDS_BYTES>();
+  const hipError_t a = allow_lds<logits_kernel<T, SPLIT, Epi>, LDS_BYTES>();
   if (a != hipSuccess) return (int)a;
-  logits_kernel<T, TERMS, Epi><<<g.ti * g.tj, WAVES * 64, LDS_BYTES, st>>>(g, epi);
+  logits_kernel<T, SPLIT, Epi><<<g.ti * g.tj, WAVES * 64, LDS_BYTES, st>>>(g, epi);
   OBMAN_LAUNCH_CHECK();
   return 0;
 }
@@ -1101,12 +1104,12 @@ static int operands(const obman_class_loss_params& p, const Keep& k, float* max_
                                                       p.ignore_index, max_part);
     OBMAN_LAUNCH_CHECK();
   }
-  const Pack px{p.x, k.xp, p.rows, k.x.rows, k.x.plane}, pw{p.w, k.wp, p.classes, k.w.rows, k.w.plane};
+  const Pack px{p.x, k.xp, p.rows, k.x.rows}, pw{p.w, k.wp, p.classes, k.w.rows};
   const long rows = px.padded > pw.padded ? px.padded : pw.padded;
-  const dim3 grid(blocks_for(rows * k.blocks * 4), 2);
-  if (p.type == F32) pack_kernel<F32><<<grid, 256, 0, st>>>(px, pw, p.width, k.blocks * 4, p.target, p.target_wide, p.ignore_index, max_part, k.scales);
-  else if (p.type == BF16) pack_kernel<BF16><<<grid, 256, 0, st>>>(px, pw, p.width, k.blocks * 4, p.target, p.target_wide, p.ignore_index, max_part, k.scales);
-  else pack_kernel<F16><<<grid, 256, 0, st>>>(px, pw, p.width, k.blocks * 4, p.target, p.target_wide, p.ignore_index, max_part, k.scales);
+  const dim3 grid(blocks_for(rows * k.ld / 8), 2);
+  if (p.type == F32) pack_kernel<F32><<<grid, 256, 0, st>>>(px, pw, p.width, k.ld / 8, p.target, p.target_wide, p.ignore_index, max_part, k.scales);
+  else if (p.type == BF16) pack_kernel<BF16><<<grid, 256, 0, st>>>(px, pw, p.width, k.ld / 8, p.target, p.target_wide, p.ignore_index, max_part, k.scales);
+  else pack_kernel<F16><<<grid, 256, 0, st>>>(px, pw, p.width, k.ld / 8, p.target, p.target_wide, p.ignore_index, max_part, k.scales);
   OBMAN_LAUNCH_CHECK();
   return 0;
 }
@@ -1122,32 +1125,30 @@ static int check(const obman_class_loss_params* p) {
 // |g| in 16 bits: scaled in fp16
 static float g_scale_of(int type) { return type == BF16 ? 1.f : G_SCALE; }
 
-template <int T, int TERMS>
+template <int T, bool SPLIT>
 static int forward(const obman_class_loss_params& p, const Keep& k, const Forward& o, hipStream_t st) {
-  constexpr bool split = TERMS == 3;
-  const Stats<split> epi{{Scale{split ? k.scales : nullptr, split ? k.scales + 1 : nullptr}, p.bias, p.type, 0, p.classes}, p.target, p.target_wide, o.part, o.picked};
-  return launch_logits<T, TERMS>(gemm_of(k.w, k.x, p.classes, p.rows, k.blocks * 32, 1, 0, 0), epi, st);
+  const Stats<SPLIT> epi{{Scale{SPLIT ? k.scales : nullptr, SPLIT ? k.scales + 1 : nullptr}, p.bias, p.type, 0, p.classes}, p.target, p.target_wide, o.part, o.picked};
+  return launch_logits<T, SPLIT>(gemm_of(k.w, k.x, p.classes, p.rows, k.ld, 1, 0, 0), epi, st);
 }
 
-template <int T, int TERMS>
+template <int T, bool SPLIT>
 static int backward(const obman_class_loss_params& p, const Keep& k, const Backward& o, const RowConst* rows, const Alpha& alpha, void* dx, void* dw, void* db, hipStream_t st) {
-  constexpr bool split = TERMS == 3;
-  const float *sx = split ? k.scales : nullptr, *sw = split ? k.scales + 1 : nullptr;
+  const float *sx = SPLIT ? k.scales : nullptr, *sw = SPLIT ? k.scales + 1 : nullptr;
   const long xr = k.x.rows;
-  const int ld = k.blocks * 32, size = p.type == F32 ? 4 : 2;
-  const hipError_t a = allow_lds<grads_kernel<T, TERMS>, LDS_BYTES>();
+  const int ld = k.ld, size = p.type == F32 ? 4 : 2;
+  const hipError_t a = allow_lds<grads_kernel<T, SPLIT>, LDS_BYTES>();
   if (a != hipSuccess) return (int)a;
   for (long v0 = 0; v0 < p.classes; v0 += o.piece) {
     const long nv = p.classes - v0 < o.piece ? p.classes - v0 : o.piece, kv = up(nv, 32);
     const bool last = v0 + nv == p.classes;
-    const Side w{k.wp + v0 * 32, k.w.plane, k.w.rows}, gs{o.g, o.g_plane, xr};
-    const Grad<T, split> ge{{Scale{sx, sw}, p.bias, p.type, v0, v0 + nv}, rows, p.rows, xr, o.g, o.g_plane, (int)kv, db ? o.sums : nullptr};
-    if (const int e = launch_logits<T, TERMS>(gemm_of(w, k.x, kv, xr, ld, 1, 0, 0), ge, st)) return e;
-    const Gemm gx = gemm_of(w, gs, ld, p.rows, kv, o.parts.x, k.blocks, 0), gw = gemm_of(k.x, gs, ld, nv, xr, o.parts.w, k.blocks, (int)(kv / 32));
+    const Side w{k.wp + v0 * 32, k.w.rows}, gs{o.g, xr};
+    const Grad<T, SPLIT> ge{{Scale{sx, sw}, p.bias, p.type, v0, v0 + nv}, rows, p.rows, xr, o.g, (int)kv, db ? o.sums : nullptr};
+    if (const int e = launch_logits<T, SPLIT>(gemm_of(w, k.x, kv, xr, ld, 1, 0, 0), ge, st)) return e;
+    const Gemm gx = gemm_of(w, gs, ld, p.rows, kv, o.parts.x, ld / Step<SPLIT>, 0), gw = gemm_of(k.x, gs, ld, nv, xr, o.parts.w, ld / Step<SPLIT>, (int)(kv / Step<SPLIT>));
     const int nx = dx ? gx.ti * gx.tj * gx.parts : 0, nw = dw ? gw.ti * gw.tj * gw.parts : 0;
     if (nx + nw) {
       const int second = o.parts.x_first ? nw : nx, first = nx + nw - second;
-      grads_kernel<T, TERMS><<<((first + 7) & ~7) + second, WAVES * 64, LDS_BYTES, st>>>(gx, Slab{o.dx_slabs, p.rows * ld, ld, v0 > 0}, nx, gw,
+      grads_kernel<T, SPLIT><<<((first + 7) & ~7) + second, WAVES * 64, LDS_BYTES, st>>>(gx, Slab{o.dx_slabs, p.rows * ld, ld, v0 > 0}, nx, gw,
                                                                                          Slab{o.dw_slabs, o.piece * ld, ld, 0}, nw, o.parts.x_first);
       OBMAN_LAUNCH_CHECK();
     }
@@ -1163,7 +1164,7 @@ static int backward(const obman_class_loss_params& p, const Keep& k, const Backw
   return 0;
 }
 
-constexpr long WHOLE_PARTS = 16384;  // tile statistics that one block joins: a second launch costs more than the idle CUs
+constexpr long WHOLE_ROWS = 512, WHOLE_PARTS = 16384;  // what one block joins: a second launch costs more than the idle CUs
 
 }  // namespace cl
 
@@ -1194,13 +1195,13 @@ int obman_class_loss_fwd(const obman_class_loss_params* p, void* keep, void* ws,
   const cl::Keep k = cl::keep_of(*p, keep ? keep : static_cast<char*>(ws) + cl::forward_of(*p, nullptr).bytes);
   const cl::Forward o = cl::forward_of(*p, ws);
   if ((e = cl::operands(*p, k, o.max_part, st))) return e;
-  e = p->type == cl::F32    ? cl::forward<cl::F16, 3>(*p, k, o, st)
-      : p->type == cl::BF16 ? cl::forward<cl::BF16, 1>(*p, k, o, st)
-                            : cl::forward<cl::F16, 1>(*p, k, o, st);
+  e = p->type == cl::F32    ? cl::forward<cl::F16, true>(*p, k, o, st)
+      : p->type == cl::BF16 ? cl::forward<cl::BF16, false>(*p, k, o, st)
+                            : cl::forward<cl::F16, false>(*p, k, o, st);
   if (e) return e;
   cl::RowConst* consts = keep && p->reduction ? k.rows : nullptr;
   const float gs = cl::g_scale_of(p->type);
-  if (p->rows * o.ti <= cl::WHOLE_PARTS) {
+  if (p->rows <= cl::WHOLE_ROWS && p->rows * o.ti <= cl::WHOLE_PARTS) {
     cl::join_rows_kernel<true><<<1, 1024, 0, st>>>(o.part, o.ti, p->rows, p->classes, o.picked, p->target, p->target_wide, p->ignore_index, p->reduction, gs, k.lse, loss,
                                                    consts, nullptr, k.norm);
     OBMAN_LAUNCH_CHECK();
@@ -1232,9 +1233,9 @@ int obman_class_loss_bwd(const obman_class_loss_params* p, const void* keep, con
     alpha = cl::Alpha{o.alpha, nullptr, 1.f / gs};
   }
   const cl::RowConst* rows = p->reduction ? k.rows : o.rows;
-  return p->type == cl::F32    ? cl::backward<cl::F16, 3>(*p, k, o, rows, alpha, dx, dw, db, st)
-         : p->type == cl::BF16 ? cl::backward<cl::BF16, 1>(*p, k, o, rows, alpha, dx, dw, db, st)
-                               : cl::backward<cl::F16, 1>(*p, k, o, rows, alpha, dx, dw, db, st);
+  return p->type == cl::F32    ? cl::backward<cl::F16, true>(*p, k, o, rows, alpha, dx, dw, db, st)
+         : p->type == cl::BF16 ? cl::backward<cl::BF16, false>(*p, k, o, rows, alpha, dx, dw, db, st)
+                               : cl::backward<cl::F16, false>(*p, k, o, rows, alpha, dx, dw, db, st);
 }
 
 }  // extern "C"
