@@ -8,8 +8,9 @@ enum { NORM_INF = 0, NORM_1 = 1, NORM_2 = 2 };
 enum { F32 = 0, BF16 = 1, F16 = 2 };
 
 constexpr int MAX_TENSORS = 192;  // per launch: 192 x 20 bytes of kernel arguments (limit 4 KB)
-constexpr int CHUNK = 4096;       // elements: 16 per thread of a 256-thread block, four 16-byte loads in flight for fp32
-constexpr int GN_BLOCKS = 1024;   // four blocks per CU; also what the join reads
+constexpr int CHUNK_BYTES = 16384;  // four 16-byte loads in flight per thread of a 256-thread block
+__host__ __device__ constexpr int chunk_of(int type) { return type == 0 ? CHUNK_BYTES / 4 : CHUNK_BYTES / 2; }
+constexpr int GN_BLOCKS = 2048;   // eight blocks per CU; also what the join reads
 constexpr int GN_SMALL_CHUNKS = 8;
 
 struct Batch {
@@ -62,15 +63,18 @@ __device__ __forceinline__ void add(float x, int norm, double& acc, unsigned& to
 template <int TYPE>
 __device__ __forceinline__ void chunk_sum16(const unsigned short* __restrict__ g, int n, int norm, int tid, int threads, double& acc, unsigned& top) {
   const int full = n & ~7;
-  for (int i = tid * 8; i < full; i += threads * 16) {
-    const int j = i + threads * 8;
-    const u16x8u a = *reinterpret_cast<const u16x8u*>(g + i);
-    u16x8u c = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (j < full) c = *reinterpret_cast<const u16x8u*>(g + j);
+  for (int i = tid * 8; i < full; i += threads * 32) {
+    u16x8u v[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) add(widen<TYPE>(a[e]), norm, acc, top);
+    for (int k = 0; k < 4; ++k) {
+      const int j = i + k * threads * 8;
+      v[k] = u16x8u{0, 0, 0, 0, 0, 0, 0, 0};
+      if (j < full) v[k] = *reinterpret_cast<const u16x8u*>(g + j);
+    }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) add(widen<TYPE>(c[e]), norm, acc, top);
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) add(widen<TYPE>(v[k][e]), norm, acc, top);
   }
   for (int i = full + tid; i < n; i += threads) add(widen<TYPE>(g[i]), norm, acc, top);
 }
@@ -104,11 +108,20 @@ __device__ __forceinline__ void chunk_sum(const void* p, int type, long at, int 
 template <int TYPE>
 __device__ __forceinline__ void chunk_scale16(unsigned short* __restrict__ g, int n, float k, int tid, int threads) {
   const int full = n & ~7;
-  for (int i = tid * 8; i < full; i += threads * 8) {
-    u16x8u a = *reinterpret_cast<u16x8u*>(g + i);
+  for (int i = tid * 8; i < full; i += threads * 32) {
+    u16x8u v[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) a[e] = narrow<TYPE>(widen<TYPE>(a[e]) * k);  // one rounding, to the gradient's own type
-    *reinterpret_cast<u16x8u*>(g + i) = a;
+    for (int q = 0; q < 4; ++q) {
+      const int j = i + q * threads * 8;
+      if (j < full) v[q] = *reinterpret_cast<u16x8u*>(g + j);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int j = i + q * threads * 8;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[q][e] = narrow<TYPE>(widen<TYPE>(v[q][e]) * k);  // one rounding, to the gradient's own type
+      if (j < full) *reinterpret_cast<u16x8u*>(g + j) = v[q];
+    }
   }
   for (int i = full + tid; i < n; i += threads) g[i] = narrow<TYPE>(widen<TYPE>(g[i]) * k);
 }
@@ -204,8 +217,9 @@ static inline int fill(Batch& b, const Get& get, int count, int& i) {
     const Item t = get(i);
     if (t.n < 0 || t.type < 0 || t.type > 2) return -2;
     if (t.n == 0) continue;
-    if (!t.p || t.n > (long)CHUNK * 0x7fffffffL) return -2;
-    const long c = b.first_chunk[b.count] + (t.n + CHUNK - 1) / CHUNK;
+    const int chunk = chunk_of(t.type);
+    if (!t.p || t.n > (long)chunk * 0x7fffffffL) return -2;
+    const long c = b.first_chunk[b.count] + (t.n + chunk - 1) / chunk;
     if (c > 0x7fffffffL) {
       if (!b.count) return -3;
       break;  // the chunk index would leave 32 bits: this tensor opens the next table

@@ -26,9 +26,10 @@ __global__ __launch_bounds__(256) void partial_kernel(Batch b, int norm, double*
   unsigned top = 0;
   for (; c < c1; ++c) {
     while (c >= b.first_chunk[t + 1]) ++t;
-    const long at = (c - b.first_chunk[t]) * CHUNK;
+    const int type = type_of(b, t), chunk = chunk_of(type);
+    const long at = (c - b.first_chunk[t]) * chunk;
     const long n = count_of(b, t) - at;
-    chunk_sum(b.p[t], type_of(b, t), at, n < CHUNK ? (int)n : CHUNK, norm, threadIdx.x, 256, acc, top);
+    chunk_sum(b.p[t], type, at, n < chunk ? (int)n : chunk, norm, threadIdx.x, 256, acc, top);
   }
   const double s = norm == NORM_INF ? (double)__uint_as_float(block_max<256>(top)) : block_sum<256>(acc);
   if (threadIdx.x == 0) part[blockIdx.x] = s;
@@ -51,9 +52,10 @@ __global__ __launch_bounds__(256) void scale_kernel(Batch b, int norm, const dou
   int t = find(b, c);
   for (; c >= c0; --c) {
     while (c < b.first_chunk[t]) --t;
-    const long at = (c - b.first_chunk[t]) * CHUNK;
+    const int type = type_of(b, t), chunk = chunk_of(type);
+    const long at = (c - b.first_chunk[t]) * chunk;
     const long n = count_of(b, t) - at;
-    chunk_scale(b.p[t], type_of(b, t), at, n < CHUNK ? (int)n : CHUNK, k, threadIdx.x, 256);
+    chunk_scale(b.p[t], type, at, n < chunk ? (int)n : chunk, k, threadIdx.x, 256);
   }
 }
 
