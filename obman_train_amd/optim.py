@@ -53,10 +53,9 @@ def _same_device(tensors, what):
             raise TypeError("%s must be fp32, bf16 or fp16, got %s" % (what, dtype))
         if d != dev:
             raise ValueError("%s must be on one device, got %s and %s" % (what, dev, d))
-    try:
-        contiguous = all(map(torch.Tensor.is_contiguous, tensors))
-    except RuntimeError:
-        raise TypeError("%s must be dense tensors" % what) from None
+    contiguous = all(map(torch.Tensor.is_contiguous, tensors))
+    if not contiguous and any(t.layout != torch.strided for t in tensors):
+        raise TypeError("%s must be dense tensors" % what)
     return dev, _GRAD_TYPES[groups[0][1]] if len(groups) == 1 else None, contiguous
 
 
