@@ -1031,7 +1031,7 @@ static Forward forward_of(const obman_class_loss_params& p, void* mem) {
 // block of unevenness.  (At 19 200 x 12 800 x 512 the measured times of ten cuts are 0.43 - 0.45 us per such step.)
 constexpr double START = 15.0, ALONE = 1.2;
 constexpr int CUS = 256;
-struct Parts { int x, w; bool x_first; };
+struct Parts { int x, w; bool x_first; double steps; };
 static double launch_steps(double n_long, double l_long, double n_short, double l_short) {
   const double n = n_long + n_short;
   if (n > 2 * CUS) {
@@ -1044,7 +1044,7 @@ static double launch_steps(double n_long, double l_long, double n_short, double 
   return first + paired;
 }
 static Parts parts_of(long tiles_x, long k_x, long tiles_w, long k_w) {
-  Parts best{1, 1, true};
+  Parts best{1, 1, true, 0.0};
   double least = 0.0;
   for (int x = 1; x <= (tiles_x ? 32 : 1); ++x) {
     if (x > 1 && k_x / x < 256) break;
@@ -1053,7 +1053,7 @@ static Parts parts_of(long tiles_x, long k_x, long tiles_w, long k_w) {
       const double lx = k_x / 32 / x + START, lw = k_w / 32 / w + START, nx = (double)tiles_x * x, nw = (double)tiles_w * w;
       const bool first = !tiles_w || (tiles_x && lx >= lw);
       const double t = first ? launch_steps(nx, lx, nw, lw) : launch_steps(nw, lw, nx, lx);
-      if (least == 0.0 || t < least) { least = t; best = {x, w, first}; }
+      if (least == 0.0 || t < least) { least = t; best = {x, w, first, t}; }
     }
   }
   return best;
@@ -1075,13 +1075,24 @@ static Backward backward_of(const obman_class_loss_params& p, const Keep& k, voi
   const long xr = k.x.rows, all = up(p.classes, 32);
   o.rows = c.take<RowConst>(p.reduction ? 0 : p.rows);
   o.alpha = c.take<float>(1);
+  const long tiles_d = obman_cdiv(ld, BI), tiles_x = need_x ? tiles_d * obman_cdiv(p.rows, BJ) : 0;
+  const auto cut = [&](long piece) { return parts_of(tiles_x, piece * terms, need_w ? tiles_d * obman_cdiv(piece, BJ) : 0, xr * terms); };
   long most = PIECE_BYTES / (xr * 2 * planes) / BI * BI;
   if (most < 2 * BI) most = 2 * BI;
   o.piece = all;
-  if (most < all) o.piece = up(all / ((all + most - 1) / most) + 1, BI);  // equal pieces
+  if (most < all) {  // equal pieces; of a few numbers of them the one whose launches fill the CUs best
+    const long least = (all + most - 1) / most;
+    double best = 0.0;
+    for (long n = least; n < least + 6; ++n) {
+      const long piece = up(all / n + 1, BI);
+      if (piece > most && n > least) continue;
+      const double t = cut(piece).steps * ((all + piece - 1) / piece);
+      if (best == 0.0 || t < best) { best = t; o.piece = piece; }
+    }
+  }
   if (o.piece > all) o.piece = all;
+  o.parts = cut(o.piece);
   o.g = c.take<u16>((size_t)planes * xr * o.piece);
-  o.parts = parts_of(need_x ? (long)obman_cdiv(ld, BI) * obman_cdiv(p.rows, BJ) : 0, o.piece * terms, need_w ? (long)obman_cdiv(ld, BI) * obman_cdiv(o.piece, BJ) : 0, xr * terms);
   o.dx_slabs = c.take<float>(need_x ? (size_t)o.parts.x * p.rows * ld : 0);
   o.dw_slabs = c.take<float>(need_w ? (size_t)o.parts.w * o.piece * ld : 0);
   o.sums = c.take<float>(need_b ? (size_t)(xr / BJ) * o.piece : 0);
