@@ -298,7 +298,7 @@ int obman_bf16_shadow(const float* src, uint16_t* dst, long n, obman_stream_t st
  * reduction: 0 per row, 1 sum, 2 mean over the rows that are not ignored (0 if there are none).
  * rows, classes: at most 2^22; width: at most 16384.
  * Forward: loss (rows floats, or one).  keep holds what the backward pass needs - it does not read x and w again; NULL (keeps = 0
- * for the sizes): none will follow, and up to 32 rows are then scored with one read of w as it is.
+ * for the sizes): none will follow, and up to 32 rows of 4 KB or 64 rows of 2 KB are then scored with one read of w as it is.
  * Backward: g_loss (rows floats, or one); dx, dw, db of the inputs' type, each may be NULL (need_* = 0 for the sizes).  The gradient
  * of the logits exists for a piece of the classes at a time, in the scratch.  Fixed summation order: the same bits every call.
  * obman_class_loss_sizes: bytes of keep and of the two calls' scratch ws, 256-byte aligned device memory. */

@@ -629,23 +629,33 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack px, Pack pw, int width, 
   }
 }
 
-// Few rows (scoring single features): the table is read once, as it is, and that read is the time.  A wave holds 32 classes x up to 32
-// rows: its lanes load 16 bytes of each of the 32 class rows straight into matrix operands (a lane's element order along the width is
-// free as long as x, staged in LDS, has the same), fp32 on the fp32 instruction.  Blocks run over the table with running statistics.
-constexpr int FEW = 32;
+// Few rows (scoring single features): the table is read once, as it is, and that read is the time.  A wave holds 32 classes x 32 G rows:
+// its lanes load 16 bytes of each of the 32 class rows straight into matrix operands (a lane's element order along the width is free
+// as long as x, staged in LDS, has the same), fp32 on the fp32 instruction.  Blocks run over the table with running statistics.
+constexpr int FEW = 64;  // most rows: at 64 050 classes x 512 in bf16, 64 take 36 us here and 60 packed, 128 would take 70 and 62
 template <int TYPE> struct FewT { static constexpr int E = 8; };  // elements of a 16-byte piece
 template <> struct FewT<F32> { static constexpr int E = 4; };
-template <int TYPE>
+template <int TYPE, int G>
 __global__ __launch_bounds__(256) void few_kernel(const void* __restrict__ xs, const void* __restrict__ ws, const void* __restrict__ bias, const void* target, int wide, int rows,
                                                  long classes, int width, float2* __restrict__ part, float* __restrict__ picked) {
-  constexpr int E = FewT<TYPE>::E, SIZE = 16 / E, AHEAD = 8;
+  constexpr int E = FewT<TYPE>::E, SIZE = 16 / E, AHEAD = 8, R = 32 * G;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ float2 red[4][FEW];
+  __shared__ float2 red[4][R];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
   const int pieces = (width + 2 * E - 1) / (2 * E);  // of 2 E columns, one 16-byte half for each half of the wave
+  const int safe = width / (2 * E);                  // pieces that lie inside the row
+  long v0 = ((long)blockIdx.x * 4 + wave) * 32;
+  const auto row_of = [&](long v) { return static_cast<const char*>(ws) + (v < classes ? v : classes - 1) * width * SIZE + half * 16; };
+  const char* row = row_of(v0 + (lane & 31));
+  u32x4 a[AHEAD];
+  const auto load = [&](int p) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) a[u] = *reinterpret_cast<const u32x4u*>(row + (p + u) * 32);
+  };
+  if (safe >= AHEAD) load(0);  // under way while x is staged
   // x in LDS: [piece][half][row] 16 bytes, zeros behind the width and the last row
-  for (int i = tid; i < pieces * 2 * FEW; i += 256) {
-    const int r = i % FEW, c = i / FEW * E;
+  for (int i = tid; i < pieces * 2 * R; i += 256) {
+    const int r = i % R, c = i / R * E;
     u32x4 v = {0, 0, 0, 0};
     if (r < rows) {
       const char* p = static_cast<const char*>(xs) + ((long)r * width + c) * SIZE;
@@ -661,71 +671,88 @@ __global__ __launch_bounds__(256) void few_kernel(const void* __restrict__ xs, c
     reinterpret_cast<u32x4*>(smem)[i] = v;
   }
   __syncthreads();
-  const char* xl = smem + (half * FEW + (lane & 31)) * 16;
-  const int r = lane & 31;
-  const long t = r < rows ? target_of(target, wide, r) : -1;
-  const int safe = width / (2 * E);  // pieces that lie inside the row
-  float m = -INFINITY, s = 0.f;
-  for (long v0 = ((long)blockIdx.x * 4 + wave) * 32; v0 < classes; v0 += (long)gridDim.x * 128) {
-    const long v = v0 + (lane & 31);
-    const char* row = static_cast<const char*>(ws) + (v < classes ? v : classes - 1) * width * SIZE + half * 16;
-    f32x16 acc;
+  const char* xl = smem + (half * R + (lane & 31)) * 16;
+  long t[G];
+  float m[G], s[G];
 #pragma unroll
-    for (int q = 0; q < 16; ++q) acc[q] = 0.f;
-    const auto step = [&](u32x4 a, int p) {
-      const u32x4 b = *reinterpret_cast<const u32x4*>(xl + p * (2 * FEW * 16));
-      if constexpr (TYPE == F32) {
+  for (int g = 0; g < G; ++g) {
+    const int r = g * 32 + (lane & 31);
+    t[g] = r < rows ? target_of(target, wide, r) : -1;
+    m[g] = -INFINITY;
+    s[g] = 0.f;
+  }
+  for (bool first = true; v0 < classes; v0 += (long)gridDim.x * 128, first = false) {
+    if (!first) {
+      row = row_of(v0 + (lane & 31));
+      if (safe >= AHEAD) load(0);
+    }
+    f32x16 acc[G];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(b[e]), acc, 0, 0, 0);
-      } else acc = mfma<TYPE>(a, b, acc);
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) acc[g][q] = 0.f;
+    const auto step = [&](u32x4 w, int p) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const u32x4 b = *reinterpret_cast<const u32x4*>(xl + (p * 2 * R + g * 32) * 16);
+        if constexpr (TYPE == F32) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[g] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(w[e]), __uint_as_float(b[e]), acc[g], 0, 0, 0);
+        } else acc[g] = mfma<TYPE>(w, b, acc[g]);
+      }
     };
     int p = 0;
     for (; p + AHEAD <= safe; p += AHEAD) {
-      u32x4 a[AHEAD];
-#pragma unroll
-      for (int u = 0; u < AHEAD; ++u) a[u] = *reinterpret_cast<const u32x4u*>(row + (p + u) * 32);
+      if (p) load(p);
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) step(a[u], p + u);
     }
     for (; p < safe; ++p) step(*reinterpret_cast<const u32x4u*>(row + p * 32), p);
     if (p < pieces) {
-      u32x4 a = {0, 0, 0, 0};
+      u32x4 w = {0, 0, 0, 0};
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const int c = p * 2 * E + half * E + e;
         if (c >= width) continue;
-        if constexpr (TYPE == F32) a[e] = reinterpret_cast<const unsigned*>(row + p * 32)[e];
-        else a[e >> 1] |= (unsigned)reinterpret_cast<const u16*>(row + p * 32)[e] << (16 * (e & 1));
+        if constexpr (TYPE == F32) w[e] = reinterpret_cast<const unsigned*>(row + p * 32)[e];
+        else w[e >> 1] |= (unsigned)reinterpret_cast<const u16*>(row + p * 32)[e] << (16 * (e & 1));
       }
-      step(a, p);
+      step(w, p);
     }
-    // lane: row lane % 32, classes v0 + 8 (q / 4) + 4 half + q % 4
-    float top = m;
+    // lane: row 32 g + lane % 32, classes v0 + 8 (q / 4) + 4 half + q % 4
 #pragma unroll
-    for (int q = 0; q < 16; ++q) {
-      const long c = v0 + 8 * (q >> 2) + 4 * half + (q & 3);
-      acc[q] = c < classes ? acc[q] + (bias ? load_one(bias, TYPE, c) : 0.f) : -INFINITY;
-      if (c == t) picked[r] = acc[q];
-      top = fmaxf(top, acc[q]);
+    for (int g = 0; g < G; ++g) {
+      float top = m[g];
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const long c = v0 + 8 * (q >> 2) + 4 * half + (q & 3);
+        acc[g][q] = c < classes ? acc[g][q] + (bias ? load_one(bias, TYPE, c) : 0.f) : -INFINITY;
+        if (c == t[g]) picked[g * 32 + (lane & 31)] = acc[g][q];
+        top = fmaxf(top, acc[g][q]);
+      }
+      const float ref = top == -INFINITY ? 0.f : top * LOG2E;
+      s[g] *= __builtin_amdgcn_exp2f(m[g] * LOG2E - ref);
+#pragma unroll
+      for (int q = 0; q < 16; ++q) s[g] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[g][q], LOG2E, -ref));
+      m[g] = top;
     }
-    const float ref = top == -INFINITY ? 0.f : top * LOG2E;
-    s *= __builtin_amdgcn_exp2f(m * LOG2E - ref);
-#pragma unroll
-    for (int q = 0; q < 16; ++q) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[q], LOG2E, -ref));
-    m = top;
   }
-  const auto join = [&](float m2, float s2) {
+  const auto join = [](float& m, float& s, float m2, float s2) {
     const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top * LOG2E;
     s = s * __builtin_amdgcn_exp2f(m * LOG2E - ref) + s2 * __builtin_amdgcn_exp2f(m2 * LOG2E - ref);
     m = top;
   };
-  join(__shfl_xor(m, 32, 64), __shfl_xor(s, 32, 64));
-  if (half == 0) red[wave][r] = make_float2(m, s);
-  __syncthreads();
-  if (wave == 0 && half == 0 && r < rows) {
 #pragma unroll
-    for (int w = 1; w < 4; ++w) join(red[w][r].x, red[w][r].y);
-    part[(long)r * gridDim.x + blockIdx.x] = make_float2(m, s);
+  for (int g = 0; g < G; ++g) {
+    join(m[g], s[g], __shfl_xor(m[g], 32, 64), __shfl_xor(s[g], 32, 64));
+    if (half == 0) red[wave][g * 32 + lane] = make_float2(m[g], s[g]);
+  }
+  __syncthreads();
+  if (tid < rows && tid < R) {
+    float2 k = red[0][tid];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) join(k.x, k.y, red[w][tid].x, red[w][tid].y);
+    part[(long)tid * gridDim.x + blockIdx.x] = k;
   }
 }
 
@@ -973,32 +1000,39 @@ static hipError_t allow_lds() {
 
 // scoring of few rows: the table is read as it is
 constexpr int FEW_BLOCKS = 512;
-constexpr size_t FEW_LDS = 128 * 1024;  // of x: width 2048 in 16 bits, 1024 in fp32
+constexpr size_t FEW_LDS = 128 * 1024;  // of x: 32 rows of 4 KB, 64 of 2 KB
 struct Few {
   float2* part;
   float *picked, *lse, *norm;
-  int blocks;
+  int blocks, groups;
   size_t bytes, lds;
 };
 static bool few_of(const obman_class_loss_params& p, void* mem, Few* o) {
   Carve c{static_cast<char*>(mem)};
-  const long groups = (p.classes + 127) / 128;
-  o->blocks = (int)(groups < FEW_BLOCKS ? groups : FEW_BLOCKS);
+  const long tiles = (p.classes + 127) / 128;
+  o->groups = p.rows <= 32 ? 1 : 2;
+  o->blocks = (int)(tiles < FEW_BLOCKS ? tiles : FEW_BLOCKS);
   o->part = c.take<float2>((size_t)o->blocks * FEW);
   o->picked = c.take<float>(FEW);
   o->lse = c.take<float>(FEW);
   o->norm = c.take<float>(1);
   o->bytes = c.at;
   const int e = p.type == F32 ? 4 : 8;
-  o->lds = (size_t)up(p.width, 2 * e) / e * FEW * 16;
+  o->lds = (size_t)up(p.width, 2 * e) / e * (32 * o->groups) * 16;
   return p.rows <= FEW && o->lds <= FEW_LDS;
+}
+template <int TYPE, int G>
+static int launch_few(const obman_class_loss_params& p, const Few& o, hipStream_t st) {
+  const hipError_t a = allow_lds<few_kernel<TYPE, G>, (int)FEW_LDS>();
+  if (a != hipSuccess) return (int)a;
+  few_kernel<TYPE, G><<<o.blocks, 256, o.lds, st>>>(p.x, p.w, p.bias, p.target, p.target_wide, (int)p.rows, p.classes, p.width, o.part, o.picked);
+  OBMAN_LAUNCH_CHECK();
+  return 0;
 }
 template <int TYPE>
 static int few(const obman_class_loss_params& p, const Few& o, float* loss, hipStream_t st) {
-  const hipError_t a = allow_lds<few_kernel<TYPE>, (int)FEW_LDS>();
-  if (a != hipSuccess) return (int)a;
-  few_kernel<TYPE><<<o.blocks, 256, o.lds, st>>>(p.x, p.w, p.bias, p.target, p.target_wide, (int)p.rows, p.classes, p.width, o.part, o.picked);
-  OBMAN_LAUNCH_CHECK();
+  const int e = o.groups == 1 ? launch_few<TYPE, 1>(p, o, st) : launch_few<TYPE, 2>(p, o, st);
+  if (e) return e;
   few_join_kernel<<<1, 1024, 0, st>>>(o.part, o.blocks, (int)p.rows, p.classes, o.picked, p.target, p.target_wide, p.ignore_index, p.reduction, loss, o.lse, o.norm);
   OBMAN_LAUNCH_CHECK();
   return 0;

@@ -150,7 +150,7 @@ def test_several_pieces_of_the_classes(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,classes,width", [(1, 1, 1), (1, 778, 512), (3, 1000, 515), (32, 5003, 100), (31, 129, 7), (17, 300, 2048), (32, 300, 1030), (33, 300, 64)])
+@pytest.mark.parametrize("rows,classes,width", [(1, 1, 1), (1, 778, 512), (3, 1000, 515), (32, 5003, 100), (31, 129, 7), (17, 300, 2048), (32, 300, 1030), (33, 300, 64), (64, 4099, 100), (65, 1000, 33), (128, 777, 512), (97, 5000, 260), (129, 300, 64)])
 def test_scoring_without_gradients(rows, classes, width, dtype):
     from obman_train_amd import ops
 
