@@ -567,7 +567,7 @@ __device__ float scale_of(const float* __restrict__ part) {
   int e = 0;
   if (m > 0.f) (void)frexpf(m, &e);  // m = f 2^e, f in [0.5, 1)
   e = 14 - e;
-  e = e > 60 ? 60 : e < -60 ? -60 : e;  // two of them multiply within fp32
+  e = e > 120 ? 120 : e < -112 ? -112 : e;  // a power of two and its inverse are normal numbers
   return m > 0.f ? ldexpf(1.f, e) : 1.f;
 }
 

@@ -138,6 +138,9 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
 
 
 class ObmanAdam(torch.optim.Adam):
+    max_grad_norm = None  # read by every step; None = no clipping
+    grad_norm = None  # 0-dim fp32 device tensor: the L2 norm of the last clipped step's gradients, before clipping
+
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, amsgrad=False, max_grad_norm=None, **kw):
         if max_grad_norm is not None and not float(max_grad_norm) >= 0.0:
             raise ValueError("max_grad_norm must not be negative or NaN, got %r" % (max_grad_norm,))
@@ -148,12 +151,14 @@ class ObmanAdam(torch.optim.Adam):
         kw.pop("foreach", None)
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=False, foreach=False, fused=False,
                          capturable=True)  # capturable: ``step`` entries are device tensors, as this kernel keeps them
-        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)  # read by every step; None = no clipping
-        self.grad_norm = None  # 0-dim fp32 device tensor: the L2 norm of the last clipped step's gradients, before clipping
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
         for group in self.param_groups:
             for p in group["params"]:
                 if not p.is_cuda or p.dtype != torch.float32:
                     raise _lib.ObmanHipError("ObmanAdam needs fp32 ROCm parameters (there is no CPU path)")
+
+    def __getstate__(self):  # copies and pickles keep the limit (torch's optimizers carry their groups and state only)
+        return dict(super().__getstate__(), max_grad_norm=self.max_grad_norm)
 
     def _init_state(self, p):
         st = self.state[p]

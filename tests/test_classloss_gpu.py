@@ -149,6 +149,63 @@ def test_several_pieces_of_the_classes(dtype):
     _close(grads[2], db, bb, dtype, "db")
 
 
+@pytest.mark.parametrize("dtype,width", [(torch.bfloat16, 512), (torch.float32, 512)])
+def test_the_most_rows_and_the_most_classes(dtype, width):
+    """2^22 rows, then 2^22 classes, 512 wide: operands of 4 and 8 GB, whose later column blocks lie beyond 2^31 bytes and 2^32 elements of
+    offset.  One more is refused."""
+    from obman_train_amd import _lib, ops
+
+    most, few = 1 << 22, 24
+    g = torch.Generator(device=DEV).manual_seed(2)
+    long = torch.empty(most, width, dtype=dtype, device=DEV)
+    for lo in range(0, most, 1 << 19):
+        long[lo:lo + (1 << 19)] = torch.randn(1 << 19, width, generator=g, device=DEV) * 0.2
+    short = (torch.randn(few, width, generator=g, device=DEV) * 0.2).to(dtype)
+    t = torch.randint(few, (most,), generator=g, device=DEV)
+    t[::5] = IGN
+    x, w = long.requires_grad_(), short.requires_grad_()
+    loss = ops.linear_cross_entropy(x, w, t, reduction="sum")
+    gx, gw = torch.autograd.grad(loss, [x, w])
+    dw, total, bw = torch.zeros(few, width, dtype=torch.float64, device=DEV), 0.0, torch.zeros(few, width, dtype=torch.float64, device=DEV)
+    for lo in range(0, most, 1 << 17):
+        s = slice(lo, lo + (1 << 17))
+        rl, lse, gr, ex, ew, _, xe, we, c, p = _exact(x[s], w, t[s], None, "sum")
+        _, px, pw, _ = _bounds(xe, we, gr, p, c, dtype, lse)
+        total += float(rl.sum())
+        dw += ew
+        bw += pw
+        if lo % (1 << 20) == 0 or lo + (1 << 17) == most:
+            _close(gx[s], ex, px, dtype, "dx from row %d" % lo)
+    assert abs(float(loss.detach()) - total) <= 1e-6 * total
+    _close(gw, dw, bw * 1.01, dtype, "dw")
+    del gx, gw
+    # the same long operand as the table of classes
+    rows = torch.randint(most, (few,), generator=g, device=DEV)
+    loss = ops.linear_cross_entropy(w, x, rows, reduction="none")
+    gw, gx = torch.autograd.grad(loss.sum(), [w, x])
+    top, acc = torch.full((few,), -math.inf, dtype=torch.float64, device=DEV), torch.zeros(few, dtype=torch.float64, device=DEV)
+    for lo in range(0, most, 1 << 17):
+        z = w.detach().double() @ x[lo:lo + (1 << 17)].detach().double().t()
+        new = torch.maximum(top, z.max(1).values)
+        acc = acc * torch.exp(top - new) + torch.exp(z - new[:, None]).sum(1)
+        top = new
+    lse = top + acc.log()
+    want = lse - (w.detach().double() * x.detach()[rows].double()).sum(1)
+    assert float((loss.detach().double() - want).abs().max()) <= 2e-5
+    for lo in (0, most // 2, most - 4096):
+        s = slice(lo, lo + 4096)
+        z = w.detach().double() @ x[s].detach().double().t()
+        pr = torch.exp(z - lse[:, None])
+        hot = (rows[:, None] == torch.arange(lo, lo + 4096, device=DEV)).double()
+        ref, mag = (pr - hot).t() @ w.detach().double(), (pr + hot).t() @ w.detach().double().abs()
+        out = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 2.0 ** -24
+        assert ((gx[s].double() - ref).abs() <= (_h(dtype) + 1e-4 * (dtype == torch.float32)) * mag + out * ref.abs() + 2.0 ** -34 * float(w.detach().abs().max())).all(), lo
+    assert torch.isfinite(gw).all()
+    del gx, gw
+    with pytest.raises(_lib.ObmanHipError):
+        ops.linear_cross_entropy(torch.empty(most + 1, 1, dtype=dtype, device=DEV), short[:, :1].detach(), torch.zeros(most + 1, dtype=torch.int64, device=DEV))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,classes,width", [(1, 1, 1), (1, 778, 512), (3, 1000, 515), (32, 5003, 100), (31, 129, 7), (17, 300, 2048), (32, 300, 1030), (33, 300, 64), (64, 4099, 100), (65, 1000, 33), (128, 777, 512), (97, 5000, 260), (129, 300, 64)])
 def test_scoring_without_gradients(rows, classes, width, dtype):
@@ -320,7 +377,7 @@ def test_empty_batch_and_shared_leaf():
     t = torch.zeros(0, dtype=torch.int64, device=DEV)
     for reduction in ("mean", "sum"):
         loss = ops.linear_cross_entropy(x, w, t, reduction=reduction)
-        assert float(loss) == 0.0
+        assert float(loss.detach()) == 0.0
         loss.backward()
         assert x.grad.shape == (0, 4)
     assert ops.linear_cross_entropy(x, w, t, reduction="none").shape == (0,)
@@ -370,6 +427,48 @@ def test_on_another_stream_and_replayed_from_a_graph():
         torch.cuda.synchronize()
         assert all(torch.equal(a.detach(), r) for a, r in zip(out, ref)), k
         eager(*_case(64, 100, 16, torch.float32, True))
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-15, 1e15])
+def test_fp32_operands_far_from_one(scale):
+    """fp32 operands are scaled by powers of two before they are split: tiny features against a huge table and the other way round."""
+    x, w, t, b = _case(90, 130, 40, torch.float32, True)
+    _check(x * scale, w / scale, t, b, "sum")
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    """Nothing is set up lazily in a way that a stream capture refuses: a fresh process records its first forward and backward."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from obman_train_amd import ops, optim
+x, w = torch.randn(300, 32, device="cuda", requires_grad=True), torch.randn(500, 32, device="cuda", requires_grad=True)
+t = torch.randint(500, (300,), device="cuda")
+y, n = torch.randn(4, 32, device="cuda"), torch.randint(500, (4,), device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    loss = ops.linear_cross_entropy(x, w, t)
+    grads = torch.autograd.grad(loss, [x, w])
+    norm = optim.grad_norm(grads)
+    with torch.no_grad():
+        score = ops.linear_cross_entropy(y, w, n)
+for _ in range(3):
+    graph.replay()
+    torch.cuda.synchronize()
+eager = ops.linear_cross_entropy(x, w, t)
+assert torch.equal(eager, loss) and all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(eager, [x, w]), grads))
+assert torch.equal(norm, optim.grad_norm(grads))
+with torch.no_grad():
+    assert torch.equal(score, ops.linear_cross_entropy(y, w, n))
+print("captured ok", flush=True)
+"""
+    root = os.path.abspath(os.path.join(os.path.dirname(__file__), ".."))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, env=dict(os.environ, PYTHONPATH=root), capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0 and "captured ok" in done.stdout, done.stdout[-2000:] + done.stderr[-2000:]
 
 
 def test_refusals():

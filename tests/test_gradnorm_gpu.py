@@ -259,6 +259,23 @@ def test_clipped_adam_state_layouts_and_shadows():
     assert float(opt.state[p]["step"]) == 4.0
 
 
+def test_a_copied_optimizer_still_clips():
+    from obman_train_amd.optim import ObmanAdam
+
+    p = torch.nn.Parameter(torch.zeros(50, device=DEV))
+    p.grad = torch.ones(50, device=DEV)
+    opt = ObmanAdam([p], lr=1e-2, max_grad_norm=0.5)
+    opt.step()
+    twin = copy.deepcopy(opt)
+    q = twin.param_groups[0]["params"][0]
+    assert twin.max_grad_norm == 0.5 and q is not p
+    for o, v in ((opt, p), (twin, q)):
+        v.grad = torch.full((50,), 2.0, device=DEV)
+        o.step()
+    assert float(twin.grad_norm) == float(opt.grad_norm) == pytest.approx(2.0 * math.sqrt(50))
+    assert torch.equal(p, q)
+
+
 def test_clipping_in_a_graph():
     """Norm, clipping and the clipped step recorded together, two graphs alive, eager work between the replays."""
     from obman_train_amd import optim
