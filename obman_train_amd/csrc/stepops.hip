@@ -59,6 +59,7 @@ __device__ __forceinline__ void adam_one(float& p, float g, float& m, float& v, 
 // the 0.001 every torch implementation multiplies by (first version: exp_avg_sq drifted from torch's by exactly that factor)
 // CLIP: the gradients are multiplied by clip[1] on their way in (they are not written back), and what depends on a tensor's step
 // count comes from adam_clip_kernel instead of two fp64 powers per thread
+// 100 M parameters: 641 us with the norm's pass, 5.0 TB/s of 3.2 GB; 13.2 M in 92 tensors: 60 us + 20 for norm and factor
 template <bool CLIP>
 __global__ __launch_bounds__(256) void adam_kernel(AdamBatch b, double lr, double beta1, double beta2, float eps, float wd,
                                                   const float* __restrict__ clip, const float2* __restrict__ corr) {

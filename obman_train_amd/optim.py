@@ -77,7 +77,6 @@ def _norm_call(tensors, dev, one_type, norm_kind, max_norm=None):
     return out
 
 
-@torch.no_grad()
 def grad_norm(tensors, norm_type=2.0):
     """The norm of all elements of all ``tensors`` (gradients, fp32 / bf16 / fp16, mixed) as one vector: a 0-dim fp32 tensor on
     their device, without a host synchronisation.  ``norm_type`` 2, 1 or inf.  Summed in 64 bits in a fixed order: bit-reproducible.
@@ -90,11 +89,10 @@ def grad_norm(tensors, norm_type=2.0):
         return torch.zeros(())
     dev, one_type, contiguous = _same_device(tensors, "tensors")
     if not contiguous:
-        tensors = [t if ops._is_dense(t) else t.contiguous() for t in tensors]
+        tensors = [t if ops._is_dense(t) else t.detach().contiguous() for t in tensors]
     return _norm_call(tensors, dev, one_type, kind)
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """``torch.nn.utils.clip_grad_norm_`` on this package's kernels: every gradient of ``parameters`` is multiplied in place by
     ``min(1, max_norm / (norm + 1e-6))`` and the norm before clipping is returned (0-dim fp32 device tensor; nothing waits for it).
@@ -129,10 +127,12 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     if odd:
         work = list(grads)
         for i in odd:
-            work[i] = grads[i].contiguous()
+            work[i] = grads[i].detach().contiguous()
     norm = _norm_call(work, dev, one_type, kind, max_norm)
-    for i in odd:
-        grads[i].copy_(work[i])
+    if odd:
+        with torch.no_grad():
+            for i in odd:
+                grads[i].copy_(work[i])
     increment_version(grads)
     return norm
 
