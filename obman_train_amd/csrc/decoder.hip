@@ -1408,7 +1408,7 @@ template <> struct L4Raw<float> {
     o[0] = f32x2v{a.x, a.y}; o[1] = f32x2v{a.z, a.w}; o[2] = f32x2v{b.x, b.y}; o[3] = f32x2v{b.z, b.w};
   }
 };
-// The per-element arithmetic runs on channel PAIRS (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32): ~17 vector instructions per
+// The per-element arithmetic runs on channel PAIRS (one instruction each where the build allows packed fp32): ~17 vector instructions per
 // element made this pass VALU-bound (r06: 118 us at R = 1.03 M rows for 263 MB of bf16 activations, 364 us at 4.1 M), the packed
 // form issues ~9.  Element-wise the operations and their order are the scalar ones.
 template <class HT>

@@ -241,7 +241,7 @@ __device__ __forceinline__ unsigned relu_bf16x2(unsigned w) {
 }
 template <>
 struct R2Fin<BGridFeatPre> {
-  // 4 v_pk_add_f32 + 4 v_cvt_pk_bf16_f32 + 4 v_pk_max_i16 per 8 elements (scalar form: 8 adds, 8 max, 4 converts)
+  // 8 adds (4 where the build allows packed fp32) + 4 v_cvt_pk_bf16_f32 + 4 v_pk_max_i16 per 8 elements (scalar form: 8 adds, 8 max, 4 converts)
   static constexpr bool PACKED = true;
   struct Pref { float4 f0, f1; };  // the k-step's LDS constants, requested one k-step ahead by the pipelined loop
   static __device__ __forceinline__ Pref pre(const BGridFeatPre&, const BGridFeatPre::Row& w, const float* fy, int Kp, int k) {
@@ -292,7 +292,7 @@ struct R2Fin<BBnRelu> {
 #pragma unroll
     for (int j = 0; j < 8; ++j) o[j] = fmaxf(__fmaf_rn(sc[j], h[j], tc[j]), 0.f);
   }
-  // packed: 4 v_pk_fma_f32 + 4 converts + 4 v_pk_max_i16 after the 8 unpacks (scalar: 8 FMAs, 8 max, 4 converts)
+  // 8 FMAs (4 where the build allows packed fp32) + 4 converts + 4 v_pk_max_i16 after the 8 unpacks (scalar: 8 FMAs, 8 max, 4 converts)
   static constexpr bool PACKED = true;
   static __device__ __forceinline__ u32x4 finp(const BBnRelu&, const BBnRelu::Row&, const float* kcs, int Kp, int k, const BBnRelu::Raw& q) {
     const float4 s0 = *reinterpret_cast<const float4*>(kcs + k), s1 = *reinterpret_cast<const float4*>(kcs + k + 4);
@@ -326,7 +326,7 @@ struct R2Fin<BGradH> {
 #pragma unroll
     for (int j = 0; j < 8; ++j) o[j] = __fmaf_rn(ka[j], gy[j], __fmaf_rn(kb[j], h[j], kc[j]));
   }
-  static constexpr bool PACKED = true;  // 8 v_pk_fma_f32 instead of 16 FMAs
+  static constexpr bool PACKED = true;  // 8 packed FMAs instead of 16 where the build allows packed fp32
   static __device__ __forceinline__ u32x4 finp(const BGradH&, const BGradH::Row&, const float* kcs, int Kp, int k, const BGradH::Raw& q) {
     const float4 a0 = *reinterpret_cast<const float4*>(kcs + k), a1 = *reinterpret_cast<const float4*>(kcs + k + 4);
     const float4 b0 = *reinterpret_cast<const float4*>(kcs + Kp + k), b1 = *reinterpret_cast<const float4*>(kcs + Kp + k + 4);

@@ -28,7 +28,8 @@ typedef unsigned long long u64;
 
 typedef float f2 __attribute__((ext_vector_type(2)));
 
-// Two queries per instruction: v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32.  Element-wise identical rounding to
+// Two queries as one vector (the library is built without packed fp32 instructions, build.py: each operation is two scalar ones; with
+// them this sweep took 124 us instead of 132 at 64 x 16 050 x 600).  Element-wise identical rounding to
 // obman_dist2 (sub, mul, fma, fma), so the scalar index-resolution pass reproduces these values bit for bit.
 __device__ __forceinline__ f2 pm_dist2_pk(f2 qx, f2 qy, f2 qz, float rx, float ry, float rz) {
   const f2 dx = qx - rx, dy = qy - ry, dz = qz - rz;
@@ -442,8 +443,8 @@ __global__ __launch_bounds__(S5_THREADS) void pairmin_s5_kernel(S5Args a) {
 #pragma unroll
     for (int k = 0; k < S5_QPT; ++k) { best[k] = __builtin_inff(); bestc[k] = 0x7fffffff; }
     const int jbeg = wave * d.slice, groups = d.slice >> 2;
-    // queries 0..3 as two packed pairs (v_pk_add / v_pk_mul / v_pk_fma: 1.8x the time of the scalar op for 2x the work,
-    // tools/ubench/valu_rate.hip), query 4 scalar; element-wise the same rounding as obman_dist2
+    // queries 0..3 as two pairs (a packed fp32 operation would take 1.8x the time of the scalar one for 2x the work,
+    // tools/ubench/valu_rate.hip; the library is built without them), query 4 scalar; element-wise the same rounding as obman_dist2
     const f2 px0 = {qx[0], qx[1]}, py0 = {qy[0], qy[1]}, pz0 = {qz[0], qz[1]};
     const f2 px1 = {qx[2], qx[3]}, py1 = {qy[2], qy[3]}, pz1 = {qz[2], qz[3]};
     auto sweep4 = [&](const float4 (&r)[4]) {  // four references against the lane's five queries: running chunk minima only
