@@ -1,7 +1,7 @@
 #!/usr/bin/env python
 """Memory-safety runs of the HIP path under the guard-page allocator (tools/efence/efence_alloc.cpp).  TEST INFRASTRUCTURE.
 
-    python tools/efence/efence.py --selftest                       # the tool itself: in-range accesses pass, 1 byte past faults
+    python tools/efence/efence.py --selftest                       # the tool itself: in-range accesses pass, 1 byte past is on a guard page
     python tools/efence/efence.py --config c3 --batch 64 --encoder-dtype bf16 --decoder-dtype bf16 --steps 2
     python tools/efence/efence.py --left ...                       # guard BEFORE every tensor instead of after it
 
@@ -75,7 +75,7 @@ def selftest_child(mode):
         assert int(t[-1]) == 0x5a
         print("[efence] selftest inside: ok", file=sys.stderr)
     elif mode == "read_past":
-        _probe(handle, t, 1, 0, sink)      # first byte past the end: must fault
+        _probe(handle, t, 1, 0, sink)      # first byte past the end: a guard page, ended on the host
         print("[efence] selftest read_past: NOT DETECTED", file=sys.stderr)
     elif mode == "write_past":
         _probe(handle, t, 1, 1, sink)
@@ -92,7 +92,7 @@ def selftest_child(mode):
 
 
 def selftest():
-    """Each case in its own process (a detected access kills it)."""
+    """Each case in its own process (a detected access ends it, before it reaches the device)."""
     ok = True
     for mode, must_die in (("inside", False), ("read_past", True), ("write_past", True), ("left_read_before", True),
                            ("write_before", True)):

@@ -231,8 +231,9 @@ void efence_stats(size_t* out5) {
 }
 }
 
-// ---- self-test: a kernel that deliberately reads / writes `beyond` bytes past the end (or before the start) of a buffer.
-// tools/efence/efence.py --selftest runs it in a child process and expects the GPU memory fault.
+// ---- self-test: one access `beyond` bytes past the end (or before the start) of a buffer.  An address that no live or parked
+// mapping holds is not touched: the process ends here, on the host, so the test shows that the guard is where the access would land
+// without a memory fault on the device.  tools/efence/efence.py --selftest runs each case in a child process.
 __global__ void efence_probe_kernel(const unsigned char* p, long n, long beyond, int write, unsigned* sink) {
   if (threadIdx.x == 0 && blockIdx.x == 0) {
     const long at = beyond >= 0 ? n - 1 + beyond : beyond;
@@ -241,6 +242,19 @@ __global__ void efence_probe_kernel(const unsigned char* p, long n, long beyond,
   }
 }
 extern "C" int efence_probe(const void* p, long n, long beyond, int write, void* sink, hipStream_t stream) {
+  const char* at = static_cast<const char*>(p) + (beyond >= 0 ? n - 1 + beyond : beyond);
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    auto holds = [at](const Rec& r) { return at >= r.map && at < r.map + r.map_bytes; };
+    bool mapped = false;
+    for (const auto& kv : live) mapped |= holds(kv.second);
+    for (const Rec& r : quarantine) mapped |= holds(r);
+    if (!mapped) {
+      fprintf(stderr, "[efence] access at %p is on a guard page: ended before the launch\n", (const void*)at);
+      fflush(stderr);
+      abort();
+    }
+  }
   efence_probe_kernel<<<1, 64, 0, stream>>>(static_cast<const unsigned char*>(p), n, beyond, write, static_cast<unsigned*>(sink));
   return (int)hipGetLastError();
 }
