@@ -663,7 +663,7 @@ def main():
             dist.init_process_group("gloo", rank=rank, world_size=world)
             collectives = stage_collectives_through_host_if_needed(dev)
         else:
-            init_rccl(dev, rank=rank, world_size=world)  # RCCL on a high-priority stream (own hardware queue)
+            init_rccl(dev, rank=rank, world_size=world)
     import warnings
     warnings.simplefilter("ignore")
     torch.backends.cudnn.benchmark = True
@@ -837,7 +837,7 @@ def main():
                 out["selftest"] = ("--backend gloo: %d ranks on %d visible device(s), collectives %s; exercises the world > 1 code "
                                    "path of this script only - `value` is not a measurement" % (world, torch.cuda.device_count(), collectives))
             out["dist"] = {"world_size": dist.get_world_size(), "backend": dist.get_backend(), "launcher_world_size": world,
-                           "rccl_high_priority_stream": not selftest, "buckets": buckets.describe(),
+                           "rccl_high_priority_stream": False, "buckets": buckets.describe(),
                            "accumulate_in_place": bool(args.dp_accumulate_in_place), "ranks": ranks_info,
                            "distinct_devices": len({(r["hostname"], r["pci_bus_id"] or r["device_uuid"] or r["device_index"])
                                                     for r in ranks_info})}

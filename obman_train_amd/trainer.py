@@ -164,7 +164,7 @@ class GraphedTrainStep:
 
     Data parallel (``buckets`` = an enabled ``dp.GradientBuckets`` on RCCL; round 5): the WHOLE step is one graph - the
     post-accumulate hooks run while the backward is being recorded, so the pack copies and the ``all_reduce`` calls (RCCL kernels
-    on RCCL's own high-priority stream, joined by events) become graph nodes in exactly the order and overlap the eager step
+    on RCCL's own stream, joined by events) become graph nodes in exactly the order and overlap the eager step
     has; ``finish()``'s waits become the join before the recorded optimizer step.  Needs a fixed autograd graph on every rank: a
     parameter without a gradient in the eager warm-up step is refused before anything is recorded (its "some rank had one" flag
     would need the host).  A host-driven backend (gloo) cannot be recorded.  (A split form for such backends - forward +
