@@ -1023,9 +1023,9 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
         raise ValueError("expected bias [classes], got %s for %d classes" % (tuple(bias.shape), weight.shape[0]))
     if weight.shape[0] == 0 or not 0 < weight.shape[1] <= 16384:
         raise ValueError("needs at least one class and a width of 1 .. 16384, got weight %s" % (tuple(weight.shape),))
-    if target.numel() == 0:  # no rows: nothing to launch; the graph stays connected
-        zero = x.float().sum() * 0.0
-        return x.float().sum(-1) if reduction == "none" else zero
+    if target.numel() == 0:  # no rows: nothing to launch; every operand stays in the graph
+        zero = x.float().sum() + weight[:0].float().sum() + (0.0 if bias is None else bias[:0].float().sum())
+        return x.float().sum(-1) + zero if reduction == "none" else zero
     x, weight, target = x.contiguous(), weight.contiguous(), target.contiguous()
     bias = None if bias is None else bias.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):

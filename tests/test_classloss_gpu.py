@@ -390,6 +390,31 @@ def test_empty_batch_and_shared_leaf():
     assert float((got - (dx + dw)).abs().max()) <= 1e-5 * float((dx + dw).abs().max())
 
 
+def test_empty_batch_of_fixed_features():
+    """No rows, and only the table learns: the loss is still differentiable and the gradients are zeros."""
+    from obman_train_amd import ops
+
+    x, t = torch.zeros(2, 0, 4, device=DEV), torch.zeros(2, 0, dtype=torch.int64, device=DEV)
+    for reduction in ("mean", "sum", "none"):
+        w, b = torch.randn(10, 4, device=DEV, requires_grad=True), torch.randn(10, device=DEV, requires_grad=True)
+        loss = ops.linear_cross_entropy(x, w, t, b, reduction=reduction)
+        assert loss.shape == ((2, 0) if reduction == "none" else ())
+        loss.sum().backward()
+        assert torch.equal(w.grad, torch.zeros_like(w)) and torch.equal(b.grad, torch.zeros_like(b))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_weights_of_many_rows(dtype):
+    """The largest weight decides the scale of all rows' gradients: in any block of 1024 rows, the last one among them; not from an
+    ignored row."""
+    for rows, at in ((8193, 8192), (9001, 0), (70001, 66666)):
+        x, w, t, b = _case(rows, 40, 24, dtype, True, 0.1)
+        g = torch.rand(rows, generator=torch.Generator().manual_seed(at)) + 0.5
+        g[at], g[at - 5] = -3e3, math.inf
+        t[at], t[at - 5] = 7, IGN
+        _check(x, w, t, b, "none", g_rows=g.to(DEV))
+
+
 def test_on_another_stream_and_replayed_from_a_graph():
     """A captured forward and backward replays to the eager results, with eager calls of other sizes between the replays."""
     from obman_train_amd import ops
