@@ -298,7 +298,7 @@ static int adam_launch(const obman_adam_tensor* tensors, int count, double lr, d
     int blocks = 0;
     for (int i = 0; i < b.count; ++i) {
       const obman_adam_tensor& t = tensors[base + i];
-      if (!t.p || !t.g || !t.m || !t.v || !t.step || t.n < 0) return -2;
+      if (t.n < 0 || !t.step || (t.n > 0 && (!t.p || !t.g || !t.m || !t.v))) return -2;  // (a tensor without elements has no memory)
       b.p[i] = t.p; b.g[i] = t.g; b.m[i] = t.m; b.v[i] = t.v; b.shadow[i] = t.shadow_bf16; b.step[i] = t.step; b.n[i] = t.n;
       b.first_block[i] = blocks;
       blocks += obman_cdiv(t.n, ADAM_CHUNK);

@@ -175,8 +175,7 @@ class ObmanAdam(torch.optim.Adam):
             with torch.enable_grad():
                 loss = closure()
         lib = _lib.lib()
-        stream = ops._stream()
-        work = []
+        work, devices = [], set()
         for gi, group in enumerate(self.param_groups):
             params = group["params"]
             grads = [p.grad for p in params]
@@ -194,20 +193,27 @@ class ObmanAdam(torch.optim.Adam):
             lr = group["lr"]
             if torch.is_tensor(lr):
                 lr = float(lr)
+            devices |= cache["devices"]
             work.append((cache["addr"], len(params), float(lr), float(b1), float(b2), float(group["eps"]), float(group["weight_decay"])))
-        if self.max_grad_norm is not None:
-            self._clipped(lib, work, stream)
+        if not work:
             return loss
-        for args in work:
-            _lib.check(lib.obman_adam_step(*args, stream), "obman_adam_step")
+        if len(devices) > 1:
+            if self.max_grad_norm is not None:
+                raise ValueError("max_grad_norm needs all parameters on one device, got %s" % sorted(map(str, devices)))
+            dev = torch.device("cuda", torch.cuda.current_device())
+        else:
+            dev, = devices
+        with ops._on_device(dev):
+            if self.max_grad_norm is not None:
+                self._clipped(lib, work, dev, ops._stream())
+            else:
+                for args in work:
+                    _lib.check(lib.obman_adam_step(*args, ops._stream()), "obman_adam_step")
         return loss
 
-    def _clipped(self, lib, work, stream):
+    def _clipped(self, lib, work, dev, stream):
         """The norm over every group's gradients, then each group's update on the clipped values.  Scratch of this call alone: recorded
         into a graph it belongs to the graph, and two graphs of one optimizer share nothing but the parameters."""
-        if not work:
-            return
-        dev = next(p for g in self.param_groups for p in g["params"] if p.grad is not None).device
         lists = (ctypes.c_void_p * len(work))(*[w[0] for w in work])
         counts = (ctypes.c_int * len(work))(*[w[1] for w in work])
         total = sum(w[1] for w in work)
@@ -218,6 +224,8 @@ class ObmanAdam(torch.optim.Adam):
         _lib.check(lib.obman_adam_norm_partials(ctypes.addressof(lists), ctypes.addressof(counts), len(work), ws.data_ptr(),
                                                 ctypes.addressof(parts), stream), "obman_adam_norm_partials")
         first = parts.value
+        if not first:
+            clip.zero_()  # gradients without elements: their norm is 0
         for args in work:
             _lib.check(lib.obman_adam_step_clipped(*args, ws.data_ptr(), first, self.max_grad_norm, clip.data_ptr(), corr.data_ptr(), stream),
                        "obman_adam_step_clipped")
@@ -227,7 +235,7 @@ class ObmanAdam(torch.optim.Adam):
     def _build(self, params):
         """The launch's descriptor table (host array of device pointers, seven words a tensor) for this set of parameters; everything but
         the gradient pointers is constant from step to step, so ``_refresh`` only rewrites those."""
-        table = array("Q")
+        table, devices = array("Q"), {p.device for p in params}
         sts, ms, vs, steps, shadows, grads = [], [], [], [], [], []
         for p in params:
             g = p.grad
@@ -252,7 +260,7 @@ class ObmanAdam(torch.optim.Adam):
                           step.data_ptr(), p.numel()))
             for to, value in ((sts, st), (ms, st["exp_avg"]), (vs, st["exp_avg_sq"]), (steps, step), (shadows, sh), (grads, g)):
                 to.append(value)
-        return {"table": table, "addr": table.buffer_info()[0], "params": list(params), "ptrs": table[0::7], "strides": [p.stride() for p in params],
+        return {"table": table, "addr": table.buffer_info()[0], "devices": devices, "params": list(params), "ptrs": table[0::7], "strides": [p.stride() for p in params],
                 "states": sts, "ms": ms, "vs": vs, "steps": steps, "shadows": shadows, "grads": grads}
 
     def _refresh(self, cache, params, grads):

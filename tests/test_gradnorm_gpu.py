@@ -326,6 +326,36 @@ def test_clipping_in_a_graph():
             assert float(again) == pytest.approx(0.25, rel=1e-4)
 
 
+def test_within_the_limit_nothing_changes():
+    """A factor of 1 leaves every bit, of many chunks and of the single block."""
+    from obman_train_amd import optim
+
+    for sizes in ([70000, 3, 40001], [5, 9]):
+        grads = _grads(sizes, TYPES["mixed"])
+        grads[0][1] = -0.0
+        keep = [g.clone() for g in grads]
+        norm = optim.clip_grad_norm_(_params(grads), 2.0 * _norm(grads, 2.0))
+        assert float(norm) == pytest.approx(_norm(keep, 2.0), rel=1e-6)
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(grads, keep))
+
+
+def test_clipped_adam_with_gradients_without_elements():
+    from obman_train_amd import optim
+
+    ps = [torch.nn.Parameter(torch.zeros(0, 3, device=DEV)), torch.nn.Parameter(torch.zeros(0, device=DEV))]
+    for p in ps:
+        p.grad = torch.zeros_like(p)
+    opt = optim.ObmanAdam(ps, max_grad_norm=1.0)
+    for _ in range(2):
+        opt.step()
+        assert float(opt.grad_norm) == 0.0
+    more = torch.nn.Parameter(torch.ones(7, device=DEV))
+    more.grad = torch.full_like(more, 2.0)
+    opt.add_param_group({"params": [more]})
+    opt.step()
+    assert float(opt.grad_norm) == pytest.approx(2.0 * math.sqrt(7.0), rel=1e-6)
+
+
 def test_on_another_stream():
     from obman_train_amd import optim
 
