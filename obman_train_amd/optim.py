@@ -42,29 +42,32 @@ def _norm_kind(norm_type):
 
 
 def _same_device(tensors, what):
-    """-> their device, the type if it is one, and whether all are contiguous.  One grouping call and C-level maps instead of a walk in
+    """-> their device, their types (numbers of the C-ABI, one for each) and whether all are contiguous.  C-level maps instead of a walk in
     Python: the checks of 92 gradients would cost more than the kernels."""
-    groups = list(torch._C._group_tensors_by_device_and_dtype([tensors], False))
-    dev = groups[0][0]
-    for d, dtype in groups:
-        if d.type != "cuda":
-            raise _lib.ObmanHipError("%s must be ROCm device tensors (the HIP path has no CPU fallback)" % what)
-        if dtype not in _GRAD_TYPES:
-            raise TypeError("%s must be fp32, bf16 or fp16, got %s" % (what, dtype))
-        if d != dev:
-            raise ValueError("%s must be on one device, got %s and %s" % (what, dev, d))
+    devices = set(map(torch.Tensor.get_device, tensors))
+    if -1 in devices:
+        raise _lib.ObmanHipError("%s must be ROCm device tensors (the HIP path has no CPU fallback)" % what)
+    if len(devices) > 1:
+        raise ValueError("%s must be on one device, got %s" % (what, ", ".join("cuda:%d" % d for d in sorted(devices))))
+    dtypes = list(map(torch.Tensor.dtype.__get__, tensors))
+    try:
+        if dtypes.count(dtypes[0]) == len(dtypes):
+            types = array("i", (_GRAD_TYPES[dtypes[0]],)) * len(dtypes)
+        else:
+            types = array("i", map(_GRAD_TYPES.__getitem__, dtypes))
+    except KeyError as e:
+        raise TypeError("%s must be fp32, bf16 or fp16, got %s" % (what, e.args[0])) from None
     contiguous = all(map(torch.Tensor.is_contiguous, tensors))
     if not contiguous and any(t.layout != torch.strided for t in tensors):
         raise TypeError("%s must be dense tensors" % what)
-    return dev, _GRAD_TYPES[groups[0][1]] if len(groups) == 1 else None, contiguous
+    return tensors[0].device, types, contiguous
 
 
-def _norm_call(tensors, dev, one_type, norm_kind, max_norm=None):
+def _norm_call(tensors, dev, types, norm_kind, max_norm=None):
     """One C-ABI call over dense tensors of one device: -> the norm, a 0-dim fp32 tensor on that device."""
     n = len(tensors)
     ptrs = array("Q", map(torch.Tensor.data_ptr, tensors))
     counts = array("q", map(torch.Tensor.numel, tensors))
-    types = array("i", [_GRAD_TYPES[t.dtype] for t in tensors]) if one_type is None else array("i", [one_type]) * n
     lib = _lib.lib()
     out = torch.empty((), dtype=torch.float32, device=dev)
     ws = torch.empty(lib.obman_grad_norm_ws_doubles(n), dtype=torch.float64, device=dev)  # of this call alone: recorded into a graph it is the graph's
@@ -87,10 +90,10 @@ def grad_norm(tensors, norm_type=2.0):
     tensors = [t for t in tensors if t is not None]
     if not tensors:
         return torch.zeros(())
-    dev, one_type, contiguous = _same_device(tensors, "tensors")
+    dev, types, contiguous = _same_device(tensors, "tensors")
     if not contiguous:
         tensors = [t if ops._is_dense(t) else t.detach().contiguous() for t in tensors]
-    return _norm_call(tensors, dev, one_type, kind)
+    return _norm_call(tensors, dev, types, kind)
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
@@ -112,7 +115,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         grads = list({id(g): g for g in grads}.values())
     if not grads:
         return torch.zeros(())
-    dev, one_type, contiguous = _same_device(grads, "gradients")
+    dev, types, contiguous = _same_device(grads, "gradients")
     odd = [] if contiguous else [i for i, g in enumerate(grads) if not ops._is_dense(g)]
     for i in odd:
         if torch._debug_has_internal_overlap(grads[i]) == 1:
@@ -128,7 +131,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         work = list(grads)
         for i in odd:
             work[i] = grads[i].detach().contiguous()
-    norm = _norm_call(work, dev, one_type, kind, max_norm)
+    norm = _norm_call(work, dev, types, kind, max_norm)
     if odd:
         with torch.no_grad():
             for i in odd:
