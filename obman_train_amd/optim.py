@@ -238,33 +238,39 @@ class ObmanAdam(torch.optim.Adam):
     def _build(self, params):
         """The launch's descriptor table (host array of device pointers, seven words a tensor) for this set of parameters; everything but
         the gradient pointers is constant from step to step, so ``_refresh`` only rewrites those."""
-        table, devices = array("Q"), {p.device for p in params}
-        sts, ms, vs, steps, shadows, grads = [], [], [], [], [], []
-        for p in params:
+        strides = list(map(torch.Tensor.stride, params))
+        sts, shadows, grads = [], [], []
+        for p, stride in zip(params, strides):
             g = p.grad
             if g.is_sparse:
                 raise RuntimeError("ObmanAdam does not support sparse gradients")
             if not ops._is_dense(p):
                 raise RuntimeError("ObmanAdam needs dense parameters (contiguous or channels_last)")
             st = self._init_state(p)
-            if st["exp_avg"].stride() != p.stride():  # a state loaded from a checkpoint written with another layout
+            if st["exp_avg"].stride() != stride:  # a state loaded from a checkpoint written with another layout
                 st["exp_avg"] = torch.empty_like(p, memory_format=torch.preserve_format).copy_(st["exp_avg"])
                 st["exp_avg_sq"] = torch.empty_like(p, memory_format=torch.preserve_format).copy_(st["exp_avg_sq"])
             step = st["step"]
             if not (torch.is_tensor(step) and step.is_cuda and step.dtype == torch.float32):
-                step = st["step"] = torch.as_tensor(float(step), dtype=torch.float32, device=p.device)
+                st["step"] = torch.as_tensor(float(step), dtype=torch.float32, device=p.device)
             sh = getattr(p, "_obman_shadow", None)
-            if sh is not None and sh.stride() != p.stride():
+            if sh is not None and sh.stride() != stride:
                 sh = p._obman_shadow = ops.bf16_shadow(p.detach())  # the parameter was re-laid out (channels_last) after the shadow was made
                 p._obman_shadow_version = p._version
-            if g.stride() != p.stride():
+            if g.stride() != stride:
                 g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)  # element order of the parameter
-            table.extend((p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), 0 if sh is None else sh.data_ptr(),
-                          step.data_ptr(), p.numel()))
-            for to, value in ((sts, st), (ms, st["exp_avg"]), (vs, st["exp_avg_sq"]), (steps, step), (shadows, sh), (grads, g)):
-                to.append(value)
-        return {"table": table, "addr": table.buffer_info()[0], "devices": devices, "params": list(params), "ptrs": table[0::7], "strides": [p.stride() for p in params],
-                "states": sts, "ms": ms, "vs": vs, "steps": steps, "shadows": shadows, "grads": grads}
+            sts.append(st)
+            shadows.append(sh)
+            grads.append(g)
+        ms, vs, steps = ([st[key] for st in sts] for key in ("exp_avg", "exp_avg_sq", "step"))
+        table = array("Q", bytes(56 * len(sts)))
+        for word, tensors in enumerate((params, grads, ms, vs, None, steps)):
+            if tensors is not None:
+                table[word::7] = array("Q", map(torch.Tensor.data_ptr, tensors))
+        table[4::7] = array("Q", (0 if sh is None else sh.data_ptr() for sh in shadows))
+        table[6::7] = array("Q", map(torch.Tensor.numel, params))
+        return {"table": table, "addr": table.buffer_info()[0], "devices": {p.device for p in params}, "params": list(params), "ptrs": table[0::7],
+                "strides": strides, "states": sts, "ms": ms, "vs": vs, "steps": steps, "shadows": shadows, "grads": grads}
 
     def _refresh(self, cache, params, grads):
         """Same parameters, same storage, same state tensors as when the table was built?  Then only the gradient pointers change.
