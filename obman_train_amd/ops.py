@@ -967,21 +967,23 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, target, ignore_index, reduction):
         loss, keep = _class_loss_forward(x, weight, bias, target, ignore_index, reduction, True)
-        ctx.save_for_backward(x, weight, bias, target, keep)
-        ctx.cfg = (ignore_index, reduction)
+        ctx.save_for_backward(bias, target, keep)  # x and weight are in keep, as the products read them
+        ctx.cfg = (x.shape, weight.shape, x.dtype, ignore_index, reduction)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss):
-        x, weight, bias, target, keep = ctx.saved_tensors
+        bias, target, keep = ctx.saved_tensors
+        x_shape, w_shape, dtype, ignore_index, reduction = ctx.cfg
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         g_loss = _dev(g_loss, "grad")
-        dev, lib = x.device, _lib.lib()
-        dx = torch.empty_like(x) if need_x else None
-        dw = torch.empty_like(weight) if need_w else None
+        dev, lib = keep.device, _lib.lib()
+        dx = torch.empty(x_shape, dtype=dtype, device=dev) if need_x else None
+        dw = torch.empty(w_shape, dtype=dtype, device=dev) if need_w else None
         db = torch.empty_like(bias) if need_b else None
-        p = _class_loss_params(x, weight, bias, target, *ctx.cfg)
+        p = _lib.ClassLossParams(None, None, _ptr(bias), target.data_ptr(), target.numel(), w_shape[0], ignore_index, w_shape[1], _CLASS_TYPES[dtype],
+                                 target.dtype == torch.int64, reduction)
         at, n = _ct.addressof(p), _SIZES()
         to = _ct.addressof(n)
         _lib.check(lib.obman_class_loss_sizes(at, 1, need_x, need_w, need_b, to, to + 8, to + 16), "obman_class_loss_sizes")

@@ -390,6 +390,27 @@ def test_empty_batch_and_shared_leaf():
     assert float((got - (dx + dw)).abs().max()) <= 1e-5 * float((dx + dw).abs().max())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_backward_after_the_operands_changed(dtype):
+    """The backward pass works on the forward pass's copies: features and table may be overwritten in between, and it may run twice."""
+    from obman_train_amd import ops
+
+    x, w, t, b = _case(300, 400, 48, dtype, True)
+    for v in (x, w, b):
+        v.requires_grad_()
+    want = torch.autograd.grad(ops.linear_cross_entropy(x, w, t, b), (x, w, b))
+    loss = ops.linear_cross_entropy(x, w, t, b)
+    with torch.no_grad():
+        x.zero_()
+        w.mul_(-3.0)
+    for _ in range(2):
+        assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(loss, (x, w, b), retain_graph=True), want))
+    with torch.no_grad():
+        b.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):  # the bias is read again
+        torch.autograd.grad(loss, (x, w, b))
+
+
 def test_empty_batch_of_fixed_features():
     """No rows, and only the table learns: the loss is still differentiable and the gradients are zeros."""
     from obman_train_amd import ops
