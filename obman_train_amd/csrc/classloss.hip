@@ -409,14 +409,36 @@ struct Grad {
   }
 };
 
-// a product's result: fp32 slabs [split][nj][ld], added to what is there or not
+// a product's result: fp32 slabs [split][nj][ld] (WIDE: the columns are i) or [split][ni][ld] (they are j), added to what is there or not
 struct Slab {
   float* out;
   long slab;
   int ld, add;
+};
+template <bool WIDE>
+struct SlabStore {
+  Slab s;
   __device__ __forceinline__ void before(const Gemm&, const Ctx&, f32x16 (&acc)[4][2]) const { clear(acc); }
   __device__ __forceinline__ void after(const Gemm& g, const Ctx& c, f32x16 (&acc)[4][2]) const {
-    float* o = out + c.split * slab;
+    float* o = s.out + c.split * s.slab;
+    const int ld = s.ld;
+    if constexpr (!WIDE) {
+#pragma unroll
+      for (int fj = 0; fj < 2; ++fj) {
+        const long j = c.j0 + c.wj * 64 + fj * 32 + (c.lane & 31);
+        if (j >= ld) continue;
+#pragma unroll
+        for (int fi = 0; fi < 4; ++fi)
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            const long i = c.i0 + c.wi * 128 + fi * 32 + (q >> 2) * 8 + 4 * (c.lane >> 5) + (q & 3);
+            if (i >= g.ni) continue;
+            float* p = o + i * ld + j;
+            *p = s.add ? acc[fi][fj][q] + *p : acc[fi][fj][q];
+          }
+      }
+      return;
+    }
 #pragma unroll
     for (int fj = 0; fj < 2; ++fj) {
       const long j = c.j0 + c.wj * 64 + fj * 32 + (c.lane & 31);
@@ -429,7 +451,7 @@ struct Slab {
           if (i >= ld) continue;
           f32x4* p = reinterpret_cast<f32x4*>(o + j * ld + i);
           f32x4 v = {acc[fi][fj][q * 4], acc[fi][fj][q * 4 + 1], acc[fi][fj][q * 4 + 2], acc[fi][fj][q * 4 + 3]};
-          if (add) v += *p;
+          if (s.add) v += *p;
           *p = v;
         }
     }
@@ -521,15 +543,16 @@ __global__ __launch_bounds__(WAVES * 64, 2) void logits_kernel(Gemm g, Epi epi) 
 
 // dx and dw of a piece of the classes in one launch (each may have no blocks): both read the same g, and their blocks fill each
 // other's last round.  The longer ones come first; first: how many blocks that is, rounded up to whole rounds of the XCDs.
-template <int T, bool SPLIT>
+// WIDE: the width is on the tile's 256 side; else on its 128 side, where 256 would leave half a tile empty (wide_of).
+template <int T, bool SPLIT, bool WIDE>
 __global__ __launch_bounds__(WAVES * 64, 2) void grads_kernel(Gemm gx, Slab ex, int nx, Gemm gw, Slab ew, int nw, int x_first) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int first = ((x_first ? nx : nw) + 7) & ~7;
   const bool is_x = ((int)blockIdx.x < first) == (x_first != 0);
   const int id = (int)blockIdx.x < first ? blockIdx.x : blockIdx.x - first;
   if (id >= (is_x ? nx : nw)) return;
-  if (is_x) gemm<true, false, T, SPLIT>(gx, ex, id, smem);
-  else gemm<true, true, T, SPLIT>(gw, ew, id, smem);
+  if (is_x) gemm<WIDE, !WIDE, T, SPLIT>(gx, SlabStore<WIDE>{ex}, id, smem);
+  else gemm<true, true, T, SPLIT>(gw, SlabStore<WIDE>{ew}, id, smem);
 }
 
 // ------------------------------------------------------------------------------------------------------- operands and rows
@@ -987,12 +1010,21 @@ struct Keep {
   int ld;  // the width, up to whole blocks
   size_t bytes;
 };
+// Which side of the tiles of dx and dw the width goes to: the 128 wide one where that leaves out 15 % of what is multiplied, whole tiles
+// counted, and the tiles are many.  Rows of g then come in 256s, each further one costing its logits and, like 512 columns, their
+// exponentials.  Forward and backward at 19 200 x 16 050: width 64 in bf16 622 -> 530 us, in fp32 1 384 -> 1 050; width 515 in fp32
+// 4 032 -> 3 820.  (At 8 000 x 4 000 x 640, 14 %: 517 -> 527; at 1 344 x 778 x 100, few tiles: 65 -> 72.)
+static bool wide_of(const obman_class_loss_params& p) {
+  const double ld = (double)up(p.width, 32), r1 = (double)up(p.rows, BJ), r2 = (double)up(p.rows, BI), v = (double)p.classes, v1 = (double)up(p.classes, BJ);
+  const double wide = up(p.width, BI) * (r1 * v + v1 * r1), tall = up(p.width, BJ) * (r2 * v + up(p.classes, BI) * r2) + (r2 - r1) * v * (ld + 512);
+  return tall > 0.85 * wide || (r1 + v1) / BJ * obman_cdiv(p.width, BI) < 128;
+}
 static Keep keep_of(const obman_class_loss_params& p, void* mem) {
   Carve c{static_cast<char*>(mem)};
   Keep k;
   const int planes = p.type == F32 ? 2 : 1;
-  const long xr = up(p.rows, BJ), wr = up(p.classes, BI);
   k.ld = (int)up(p.width, 32);
+  const long xr = up(p.rows, wide_of(p) ? BJ : BI), wr = up(p.classes, BI);  // (x has the rows of g)
   k.scales = c.take<float>(4);
   k.norm = k.scales + 2;
   k.lse = c.take<float>(p.rows);
@@ -1128,8 +1160,9 @@ static Backward backward_of(const obman_class_loss_params& p, const Keep& k, voi
   o.rows = c.take<RowConst>(p.reduction ? 0 : p.rows);
   o.alpha = c.take<float>(1);
   o.row_max = c.take<float>(p.reduction ? 0 : ROW_MAX_BLOCKS);
-  const long tiles_d = obman_cdiv(ld, BI), tiles_x = need_x ? tiles_d * obman_cdiv(p.rows, BJ) : 0;
-  const auto cut = [&](long piece) { return parts_of(tiles_x, piece * terms, need_w ? tiles_d * obman_cdiv(piece, BJ) : 0, xr * terms); };
+  const int of_width = wide_of(p) ? BI : BJ, of_rows = BI + BJ - of_width;
+  const long tiles_d = obman_cdiv(ld, of_width), tiles_x = need_x ? tiles_d * obman_cdiv(p.rows, of_rows) : 0;
+  const auto cut = [&](long piece) { return parts_of(tiles_x, piece * terms, need_w ? tiles_d * obman_cdiv(piece, of_rows) : 0, xr * terms); };
   long most = PIECE_BYTES / (xr * 2 * planes) / BI * BI;
   if (most < 2 * BI) most = 2 * BI;
   o.piece = all;
@@ -1203,12 +1236,12 @@ static int forward(const obman_class_loss_params& p, const Keep& k, const Forwar
   return launch_logits<T, SPLIT>(gemm_of(k.w, k.x, p.classes, p.rows, k.ld, 1, 0, 0), epi, st);
 }
 
-template <int T, bool SPLIT>
+template <int T, bool SPLIT, bool WIDE>
 static int backward(const obman_class_loss_params& p, const Keep& k, const Backward& o, const RowConst* rows, const Alpha& alpha, void* dx, void* dw, void* db, hipStream_t st) {
   const float *sx = SPLIT ? k.scales : nullptr, *sw = SPLIT ? k.scales + 1 : nullptr;
   const long xr = k.x.rows;
   const int ld = k.ld, size = p.type == F32 ? 4 : 2;
-  const hipError_t a = allow_lds<grads_kernel<T, SPLIT>, LDS_BYTES>();
+  const hipError_t a = allow_lds<grads_kernel<T, SPLIT, WIDE>, LDS_BYTES>();
   if (a != hipSuccess) return (int)a;
   for (long v0 = 0; v0 < p.classes; v0 += o.piece) {
     const long nv = p.classes - v0 < o.piece ? p.classes - v0 : o.piece, kv = up(nv, 32);
@@ -1216,12 +1249,14 @@ static int backward(const obman_class_loss_params& p, const Keep& k, const Backw
     const Side w{k.wp + v0 * 32, k.w.rows}, gs{o.g, xr};
     const Grad<T, SPLIT> ge{{Scale{sx, sw}, p.bias, p.type, v0, v0 + nv}, rows, p.rows, xr, o.g, (int)kv, db ? o.sums : nullptr};
     if (const int e = launch_logits<T, SPLIT>(gemm_of(w, k.x, kv, xr, ld, 1, 0, 0), ge, st)) return e;
-    const Gemm gx = gemm_of(w, gs, ld, p.rows, kv, o.parts.x, ld / Step<SPLIT>, 0), gw = gemm_of(k.x, gs, ld, nv, xr, o.parts.w, ld / Step<SPLIT>, (int)(kv / Step<SPLIT>));
+    const int d = ld / Step<SPLIT>, v = (int)(kv / Step<SPLIT>);  // column blocks of the operands and of g
+    const Gemm gx = WIDE ? gemm_of(w, gs, ld, p.rows, kv, o.parts.x, d, 0) : gemm_of(gs, w, p.rows, ld, kv, o.parts.x, 0, d);
+    const Gemm gw = WIDE ? gemm_of(k.x, gs, ld, nv, xr, o.parts.w, d, v) : gemm_of(gs, k.x, nv, ld, xr, o.parts.w, v, d);
     const int nx = dx ? gx.ti * gx.tj * gx.parts : 0, nw = dw ? gw.ti * gw.tj * gw.parts : 0;
     if (nx + nw) {
       const int second = o.parts.x_first ? nw : nx, first = nx + nw - second;
-      grads_kernel<T, SPLIT><<<((first + 7) & ~7) + second, WAVES * 64, LDS_BYTES, st>>>(gx, Slab{o.dx_slabs, p.rows * ld, ld, v0 > 0}, nx, gw,
-                                                                                         Slab{o.dw_slabs, o.piece * ld, ld, 0}, nw, o.parts.x_first);
+      grads_kernel<T, SPLIT, WIDE><<<((first + 7) & ~7) + second, WAVES * 64, LDS_BYTES, st>>>(gx, Slab{o.dx_slabs, p.rows * ld, ld, v0 > 0}, nx, gw,
+                                                                                               Slab{o.dw_slabs, o.piece * ld, ld, 0}, nw, o.parts.x_first);
       OBMAN_LAUNCH_CHECK();
     }
     const Finish fx{o.dx_slabs, o.parts.x, p.rows * ld, dx && last ? p.rows : 0, sw, dx};
@@ -1314,9 +1349,13 @@ int obman_class_loss_bwd(const obman_class_loss_params* p, const void* keep, con
     alpha = cl::Alpha{o.alpha, nullptr, 1.f / gs};
   }
   const cl::RowConst* rows = p->reduction ? k.rows : o.rows;
-  return p->type == cl::F32    ? cl::backward<cl::F16, true>(*p, k, o, rows, alpha, dx, dw, db, st)
-         : p->type == cl::BF16 ? cl::backward<cl::BF16, false>(*p, k, o, rows, alpha, dx, dw, db, st)
-                               : cl::backward<cl::F16, false>(*p, k, o, rows, alpha, dx, dw, db, st);
+  if (cl::wide_of(*p))
+    return p->type == cl::F32    ? cl::backward<cl::F16, true, true>(*p, k, o, rows, alpha, dx, dw, db, st)
+           : p->type == cl::BF16 ? cl::backward<cl::BF16, false, true>(*p, k, o, rows, alpha, dx, dw, db, st)
+                                 : cl::backward<cl::F16, false, true>(*p, k, o, rows, alpha, dx, dw, db, st);
+  return p->type == cl::F32    ? cl::backward<cl::F16, true, false>(*p, k, o, rows, alpha, dx, dw, db, st)
+         : p->type == cl::BF16 ? cl::backward<cl::BF16, false, false>(*p, k, o, rows, alpha, dx, dw, db, st)
+                               : cl::backward<cl::F16, false, false>(*p, k, o, rows, alpha, dx, dw, db, st);
 }
 
 }  // extern "C"

@@ -391,6 +391,13 @@ def test_empty_batch_and_shared_leaf():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,classes,width", [(16500, 70, 33), (250, 16400, 64), (16641, 300, 300), (16385, 1, 5), (9001, 8003, 40), (66000, 4501, 40)])
+def test_narrow_tables(rows, classes, width, dtype):
+    """Widths that leave more of a 256 wide tile empty than of a 128 wide one, at sizes with tiles enough to mind; the last in pieces."""
+    _check(*_case(rows, classes, width, dtype, True, 0.1), "mean", scale=float(rows))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_backward_after_the_operands_changed(dtype):
     """The backward pass works on the forward pass's copies: features and table may be overwritten in between, and it may run twice."""
     from obman_train_amd import ops
