@@ -940,57 +940,50 @@ class _on_device:
             self.ctx.__exit__(*exc)
 
 
-def _class_loss_params(x, weight, bias, target, ignore_index, reduction):
-    return _lib.ClassLossParams(x.data_ptr(), weight.data_ptr(), _ptr(bias), target.data_ptr(), target.numel(), weight.shape[0], ignore_index,
-                                weight.shape[1], _CLASS_TYPES[weight.dtype], target.dtype == torch.int64, reduction)
-
-
 _SIZES = _ct.c_long * 3
 
 
-def _class_loss_forward(x, weight, bias, target, ignore_index, reduction, keeps):
-    """-> loss, and with ``keeps`` what the backward pass needs.  All scratch is of this call alone: recorded into a graph it is the graph's."""
+def _class_loss_forward(x, weight, bias, target, ignore_index, reduction, keeps, need=(False, False, False)):
+    """-> loss, and with ``keeps`` what the backward pass needs: its copies of the operands, the call's parameters, the size of its scratch.
+    All scratch is of this call alone: recorded into a graph it is the graph's."""
     dev, lib = x.device, _lib.lib()
-    p = _class_loss_params(x, weight, bias, target, ignore_index, reduction)
+    p = _lib.ClassLossParams(x.data_ptr(), weight.data_ptr(), _ptr(bias), target.data_ptr(), target.numel(), weight.shape[0], ignore_index,
+                             weight.shape[1], _CLASS_TYPES[weight.dtype], target.dtype == torch.int64, reduction)
     at, n = _ct.addressof(p), _SIZES()
     to = _ct.addressof(n)
-    _lib.check(lib.obman_class_loss_sizes(at, int(keeps), 0, 0, 0, to, to + 8, to + 16), "obman_class_loss_sizes")
+    _lib.check(lib.obman_class_loss_sizes(at, keeps, *need, to, to + 8, to + 16), "obman_class_loss_sizes")
     loss = torch.empty(target.shape if reduction == 0 else (), dtype=torch.float32, device=dev)
     keep = torch.empty(n[0], dtype=torch.uint8, device=dev) if keeps else None
     ws = torch.empty(n[1], dtype=torch.uint8, device=dev)
     with _on_device(dev):
         _lib.check(lib.obman_class_loss_fwd(at, _ptr(keep), ws.data_ptr(), loss.data_ptr(), _stream()), "obman_class_loss_fwd")
-    return loss, keep
+    return loss, keep, p, n[2]
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, target, ignore_index, reduction):
-        loss, keep = _class_loss_forward(x, weight, bias, target, ignore_index, reduction, True)
+        loss, keep, p, ws_bytes = _class_loss_forward(x, weight, bias, target, ignore_index, reduction, True, ctx.needs_input_grad[:3])
         ctx.save_for_backward(bias, target, keep)  # x and weight are in keep, as the products read them
-        ctx.cfg = (x.shape, weight.shape, x.dtype, ignore_index, reduction)
+        ctx.cfg = (x.shape, weight.shape, x.dtype, p, ws_bytes)  # made here: autograd's thread finds Python's caches cold
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss):
         bias, target, keep = ctx.saved_tensors
-        x_shape, w_shape, dtype, ignore_index, reduction = ctx.cfg
+        x_shape, w_shape, dtype, p, ws_bytes = ctx.cfg
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         g_loss = _dev(g_loss, "grad")
-        dev, lib = keep.device, _lib.lib()
+        dev = keep.device
         dx = torch.empty(x_shape, dtype=dtype, device=dev) if need_x else None
         dw = torch.empty(w_shape, dtype=dtype, device=dev) if need_w else None
         db = torch.empty_like(bias) if need_b else None
-        p = _lib.ClassLossParams(None, None, _ptr(bias), target.data_ptr(), target.numel(), w_shape[0], ignore_index, w_shape[1], _CLASS_TYPES[dtype],
-                                 target.dtype == torch.int64, reduction)
-        at, n = _ct.addressof(p), _SIZES()
-        to = _ct.addressof(n)
-        _lib.check(lib.obman_class_loss_sizes(at, 1, need_x, need_w, need_b, to, to + 8, to + 16), "obman_class_loss_sizes")
-        ws = torch.empty(n[2], dtype=torch.uint8, device=dev)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        p.bias, p.target = _ptr(bias), target.data_ptr()  # (what hooks of saved tensors gave back; x and w are not read)
         with _on_device(dev):
-            _lib.check(lib.obman_class_loss_bwd(at, keep.data_ptr(), g_loss.data_ptr(), ws.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), _stream()),
-                       "obman_class_loss_bwd")
+            _lib.check(_lib.lib().obman_class_loss_bwd(_ct.addressof(p), keep.data_ptr(), g_loss.data_ptr(), ws.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db),
+                                                       _stream()), "obman_class_loss_bwd")
         return dx, dw, db, None, None, None
 
 
@@ -1011,9 +1004,9 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
     for name, t in (("x", x), ("weight", weight), ("target", target), ("bias", bias)):
         if t is None and name == "bias":
             continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        if not isinstance(t, torch.Tensor) or t.get_device() < 0:
             raise _lib.ObmanHipError("%s must be a ROCm device tensor (the HIP path has no CPU fallback)" % name)
-        if t.device != x.device:
+        if t.get_device() != x.get_device():
             raise ValueError("x, weight, target and bias must be on one device, got %s and %s" % (x.device, t.device))
     if x.dtype not in _CLASS_TYPES or weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
         raise TypeError("x, weight and bias must all be fp32, bf16 or fp16, got %s, %s, %s" % (x.dtype, weight.dtype, None if bias is None else bias.dtype))
