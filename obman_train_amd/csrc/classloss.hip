@@ -43,7 +43,8 @@ enum { F32 = 0, BF16 = 1, F16 = 2 };
 // are padded with zeros to whole tiles, so no address leaves an operand.
 // Tile 256 x 128, four waves of 128 x 64.  72 KB of LDS, so two blocks share a CU and one's epilogue and waits run under the other's
 // products.  (256 x 256 with eight waves, four steps deep, one block on a CU, fetches a third less; at 19 200 x 64 050 x 512 it
-// measured 1 474 us for the forward product against 1 330, 328 against 304 for g, 290 against 300 and 250 against 253 for the other two.)
+// measured 1 474 us for the forward product against 1 330, 328 against 304 for g, 290 against 300 and 250 against 253 for the other two;
+// with four waves of 128 x 128, the next half step's reads under the products, the other two together took 499 against 478.)
 constexpr int BI = 256, BJ = 128, WAVES = 4, STAGES = 3;
 constexpr int A_BYTES = BI * 64, STAGE_BYTES = A_BYTES + BJ * 64;
 constexpr int BIAS_AT = STAGES * STAGE_BYTES, LDS_BYTES = BIAS_AT + BI * 4;
