@@ -69,8 +69,9 @@ struct Gemm {
 };
 
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, unsigned lds, unsigned voff) {
-  // lane l writes 16 bytes at lds + 16 l
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(r) : "memory", "m0");
+  // lane l writes 16 bytes at lds + 16 l; a load to LDS must not be the instruction behind the write of m0: one wait state, which the
+  // compiler inserts for its own loads but not inside an asm statement
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(r) : "memory", "m0");
 }
 
 // One operand's tile for a step of Step<SPLIT> k, R (i or j) wide, in 64-byte rows of LDS.  KC: the rows are i or j and their columns
