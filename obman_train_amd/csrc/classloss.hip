@@ -258,6 +258,32 @@ __device__ __forceinline__ int target_at(long target, long first_class, int lane
   return t >= 0 && t < 128 && !(t & 4) ? (int)t : -1;
 }
 
+// Statistics of a set of logits are (m, s): the maximum, and the sum of exp(z - m).  exp is 2^(z log2 e - m log2 e) in one multiply-add, and
+// what rounding m log2 e put into every term is taken out of the sum.  That holds while the rounding is small: for |m| beyond FAR (classes
+// masked with a large negative number leave such maxima; past 2.4e38 m log2 e would not even be finite) the difference comes first.
+constexpr float FAR = 1048576.f;
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) > FAR; }
+// sum of exp(z(i) - m), i < N; m: the largest of them, 0 where that is -inf
+template <int N, class Z>
+__device__ __forceinline__ float sum_exp(const Z& z, float m) {
+  float part[4] = {0.f, 0.f, 0.f, 0.f};
+  if (__any(is_far(m))) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) part[i & 3] += __builtin_amdgcn_exp2f((z(i) - m) * LOG2E);
+    return (part[0] + part[1]) + (part[2] + part[3]);
+  }
+  const float ref = m * LOG2E;
+#pragma unroll
+  for (int i = 0; i < N; ++i) part[i & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(z(i), LOG2E, -ref));
+  return ((part[0] + part[1]) + (part[2] + part[3])) * __builtin_amdgcn_exp2f(-__builtin_fmaf(m, LOG2E, -ref));
+}
+// (m, s) <- (m, s) with (m2, s2)
+__device__ __forceinline__ void join_stats(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top;
+  s = s * __builtin_amdgcn_exp2f((m - ref) * LOG2E) + s2 * __builtin_amdgcn_exp2f((m2 - ref) * LOG2E);
+  m = top;
+}
+
 // forward: per row (j) and tile of classes (i) the maximum and the sum of exponentials
 template <bool SPLIT>
 struct Stats {
@@ -289,13 +315,7 @@ struct Stats {
 #pragma unroll
         for (int q = 0; q < 16; q += 2) top = fmaxf(top, fmaxf(acc[fi][fj][q], acc[fi][fj][q + 1]));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float ref = top == -INFINITY ? 0.f : top * LOG2E;
-      float part4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int fi = 0; fi < 4; ++fi)
-#pragma unroll
-        for (int q = 0; q < 16; ++q) part4[q & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[fi][fj][q], LOG2E, -ref));
-      float total = (part4[0] + part4[1]) + (part4[2] + part4[3]);
+      float total = sum_exp<64>([&](int i) { return acc[i >> 4][fj][i & 15]; }, top == -INFINITY ? 0.f : top);
       total += __shfl_xor(total, 32, 64);
       m[fj] = top;
       sum[fj] = total;
@@ -307,20 +327,24 @@ struct Stats {
       for (int fj = 0; fj < 2; ++fj) {
         const long r = c.j0 + c.wj * 64 + fj * 32 + c.lane;
         const float2 o = red[c.wj * 64 + fj * 32 + c.lane];
-        const float top = fmaxf(m[fj], o.x), ref = top == -INFINITY ? 0.f : top * LOG2E;
-        const float total = sum[fj] * __builtin_amdgcn_exp2f(m[fj] * LOG2E - ref) + o.y * __builtin_amdgcn_exp2f(o.x * LOG2E - ref);
-        if (r < g.nj) part[(long)c.ti_index * g.nj + r] = make_float2(top, total);
+        join_stats(m[fj], sum[fj], o.x, o.y);
+        if (r < g.nj) part[(long)c.ti_index * g.nj + r] = make_float2(m[fj], sum[fj]);
       }
     }
   }
 };
 
 struct RowConst {  // per row of the backward pass
-  float lse2;      // (lse - log |c|) in units of log 2, +inf for a row without a gradient: g = exp2(z - lse2) is p |c| in one step
+  float lse2;      // (lse - shift - log |c|) in units of log 2, +inf for a row without a gradient: g = exp2(z - shift - lse2) is p |c| in one step
   float c;
   int target;      // -1: none
-  int pad;
+  float shift;     // the row's maximum where that is far from 0, else 0
 };
+// of a row whose statistics are m and log2 s
+__device__ __forceinline__ RowConst row_const(float m, float log_s, float c, int target) {
+  return is_far(m) ? RowConst{log_s - log2f(fabsf(c)), c, target, m} : RowConst{__builtin_fmaf(m, LOG2E, log_s) - log2f(fabsf(c)), c, target, 0.f};
+}
+constexpr RowConst NO_ROW = {INFINITY, 0.f, -1, 0.f};
 
 // backward: g of a piece of the classes, blocks of 32 classes like every operand; its column sums over the tile's rows on request
 template <int T, bool SPLIT>
@@ -337,9 +361,15 @@ struct Grad {
 #pragma unroll
     for (int fj = 0; fj < 2; ++fj) {
       const long r = c.j0 + c.wj * 64 + fj * 32 + (c.lane & 31);
-      RowConst k = {INFINITY, 0.f, -1, 0};
+      RowConst k = NO_ROW;
       if (r < n_rows) k = rows[r];
       const int t = target_at(k.target, bias.class0 + c.i0 + c.wi * 128, c.lane);
+      if (__any(k.shift != 0.f)) {
+#pragma unroll
+        for (int fi = 0; fi < 4; ++fi)
+#pragma unroll
+          for (int q = 0; q < 16; ++q) acc[fi][fj][q] -= k.shift;
+      }
 #pragma unroll
       for (int fi = 0; fi < 4; ++fi)
 #pragma unroll
@@ -761,35 +791,29 @@ __global__ __launch_bounds__(256) void few_kernel(const void* __restrict__ xs, c
         if (c == t[g]) picked[g * 32 + (lane & 31)] = acc[g][q];
         top = fmaxf(top, acc[g][q]);
       }
-      const float ref = top == -INFINITY ? 0.f : top * LOG2E;
-      s[g] *= __builtin_amdgcn_exp2f(m[g] * LOG2E - ref);
-#pragma unroll
-      for (int q = 0; q < 16; ++q) s[g] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[g][q], LOG2E, -ref));
+      const float ref = top == -INFINITY ? 0.f : top;
+      s[g] = s[g] * __builtin_amdgcn_exp2f((m[g] - ref) * LOG2E) + sum_exp<16>([&](int q) { return acc[g][q]; }, ref);
       m[g] = top;
     }
   }
-  const auto join = [](float& m, float& s, float m2, float s2) {
-    const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top * LOG2E;
-    s = s * __builtin_amdgcn_exp2f(m * LOG2E - ref) + s2 * __builtin_amdgcn_exp2f(m2 * LOG2E - ref);
-    m = top;
-  };
 #pragma unroll
   for (int g = 0; g < G; ++g) {
-    join(m[g], s[g], __shfl_xor(m[g], 32, 64), __shfl_xor(s[g], 32, 64));
+    join_stats(m[g], s[g], __shfl_xor(m[g], 32, 64), __shfl_xor(s[g], 32, 64));
     if (half == 0) red[wave][g * 32 + lane] = make_float2(m[g], s[g]);
   }
   __syncthreads();
   if (tid < rows && tid < R) {
     float2 k = red[0][tid];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) join(k.x, k.y, red[w][tid].x, red[w][tid].y);
+    for (int w = 1; w < 4; ++w) join_stats(k.x, k.y, red[w][tid].x, red[w][tid].y);
     part[(long)tid * gridDim.x + blockIdx.x] = k;
   }
 }
 
-// a row's loss from its log-sum-exp
-__device__ __forceinline__ float row_loss(float lse, long t, long classes, long ignore, const float* picked, long r) {
-  return t == ignore ? 0.f : lse - (t >= 0 && t < classes ? picked[r] : 0.f);
+// a row's loss from its statistics: the label's distance from the maximum first, log s may be lost beside either.  A label outside the
+// table poisons the loss instead of being read
+__device__ __forceinline__ float row_loss(float m, float log_s, long t, long classes, long ignore, const float* picked, long r) {
+  return t == ignore ? 0.f : t >= 0 && t < classes ? (m - picked[r]) + LN2 * log_s : NAN;
 }
 // loss = sum or mean over the kept rows (no row kept: 0); norm = what a row's gradient is multiplied by
 __device__ __forceinline__ void total_loss(double l, double k, int mean, float* loss, float* norm) {
@@ -800,25 +824,17 @@ __device__ __forceinline__ void total_loss(double l, double k, int mean, float* 
 
 // the end of few_kernel: a wave joins a row's block statistics, one block everything
 __global__ __launch_bounds__(1024) void few_join_kernel(const float2* __restrict__ part, int n, int rows, long classes, const float* __restrict__ picked, const void* target, int wide,
-                                                       long ignore, int reduction, float* __restrict__ loss, float* __restrict__ lse, float* __restrict__ norm) {
+                                                       long ignore, int reduction, float* __restrict__ loss, float* __restrict__ norm) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   __shared__ double2 red[FEW];
   for (int r = wave; r < rows; r += 16) {
     float m = -INFINITY, s = 0.f;
-    const auto join = [&](float m2, float s2) {
-      const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top * LOG2E;
-      s = s * __builtin_amdgcn_exp2f(m * LOG2E - ref) + s2 * __builtin_amdgcn_exp2f(m2 * LOG2E - ref);
-      m = top;
-    };
-    for (int i = lane; i < n; i += 64) { const float2 p = part[(long)r * n + i]; join(p.x, p.y); }
+    for (int i = lane; i < n; i += 64) { const float2 p = part[(long)r * n + i]; join_stats(m, s, p.x, p.y); }
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) join(__shfl_xor(m, off, 64), __shfl_xor(s, off, 64));
+    for (int off = 32; off > 0; off >>= 1) join_stats(m, s, __shfl_xor(m, off, 64), __shfl_xor(s, off, 64));
     const long t = target_of(target, wide, r);
-    float z = m + LN2 * __builtin_amdgcn_logf(s);
-    if (t != ignore && (t < 0 || t >= classes)) z = NAN;
-    const float l = row_loss(z, t, classes, ignore, picked, r);
+    const float l = row_loss(m, __builtin_amdgcn_logf(s), t, classes, ignore, picked, r);  // v_log_f32: log2
     if (lane == 0) {
-      lse[r] = z;
       if (reduction == 0) loss[r] = l;
       red[r] = make_double2(l, t != ignore);
     }
@@ -835,7 +851,7 @@ __global__ __launch_bounds__(1024) void few_join_kernel(const float2* __restrict
 // block of 64 rows the sum of losses and the number of kept rows.  WHOLE: one block does all rows and the reduction.
 template <bool WHOLE>
 __global__ __launch_bounds__(WHOLE ? 1024 : 256) void join_rows_kernel(const float2* __restrict__ part, int tiles, long rows, long classes, const float* __restrict__ picked,
-                                                                      const void* target, int wide, long ignore, int reduction, float g_scale, float* __restrict__ lse,
+                                                                      const void* target, int wide, long ignore, int reduction, float g_scale, float2* __restrict__ lse,
                                                                       float* __restrict__ loss, RowConst* __restrict__ consts, double2* __restrict__ sums, float* __restrict__ norm) {
   constexpr int GROUPS = WHOLE ? 4 : 1;  // of 64 rows x 4 threads
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave & 3, group = wave >> 2;
@@ -844,11 +860,7 @@ __global__ __launch_bounds__(WHOLE ? 1024 : 256) void join_rows_kernel(const flo
   for (long r0 = (long)blockIdx.x * 64; r0 < rows; r0 += WHOLE ? 256 : rows) {  // (not WHOLE: once)
     const long r = r0 + group * 64 + lane;
     float m = -INFINITY, s = 0.f;
-    const auto join = [&](float2 p) {
-      const float top = fmaxf(m, p.x), ref = top == -INFINITY ? 0.f : top * LOG2E;
-      s = s * __builtin_amdgcn_exp2f(m * LOG2E - ref) + p.y * __builtin_amdgcn_exp2f(p.x * LOG2E - ref);
-      m = top;
-    };
+    const auto join = [&](float2 p) { join_stats(m, s, p.x, p.y); };
     if (r < rows)
       for (int t = w; t < tiles; t += 4) join(part[(long)t * rows + r]);
     red[group][w][lane] = make_float2(m, s);
@@ -857,15 +869,12 @@ __global__ __launch_bounds__(WHOLE ? 1024 : 256) void join_rows_kernel(const flo
 #pragma unroll
       for (int k = 1; k < 4; ++k) join(red[group][k][lane]);
       const long t = target_of(target, wide, r);
-      float z = m + LN2 * __builtin_amdgcn_logf(s);  // v_log_f32: log2
-      if (t != ignore && (t < 0 || t >= classes)) z = NAN;  // a label outside the table poisons the loss instead of being read
-      lse[r] = z;
-      const float row = row_loss(z, t, classes, ignore, picked, r);
+      const bool none = t == ignore, outside = t < 0 || t >= classes;
+      const float log_s = !none && outside ? NAN : __builtin_amdgcn_logf(s);  // v_log_f32: log2
+      lse[r] = make_float2(m, log_s);
+      const float row = row_loss(m, log_s, t, classes, ignore, picked, r);
       if (reduction == 0) loss[r] = row;
-      if (consts) {
-        const bool none = t == ignore;
-        consts[r] = RowConst{none ? INFINITY : z * LOG2E - log2f(g_scale), none ? 0.f : g_scale, none || t < 0 || t >= classes ? -1 : (int)t, 0};
-      }
+      if (consts) consts[r] = none ? NO_ROW : row_const(m, log_s, g_scale, outside ? -1 : (int)t);
       l += row;
       kept += t != ignore;
     }
@@ -923,7 +932,7 @@ __global__ __launch_bounds__(1024) void row_max_kernel(const void* target, int w
 
 // A gradient for every row: RowConst with its weight, scaled to at most 1 in magnitude by a power of two; alpha takes it back.  part: the
 // ROW_MAX_BLOCKS maxima of row_max_kernel, or NULL: every block looks through all rows.
-__global__ __launch_bounds__(1024) void rows_kernel(const float* __restrict__ lse, const void* target, int wide, long ignore, long rows, const float* __restrict__ g_loss,
+__global__ __launch_bounds__(1024) void rows_kernel(const float2* __restrict__ lse, const void* target, int wide, long ignore, long rows, const float* __restrict__ g_loss,
                                                    const float* __restrict__ part, float g_scale, RowConst* __restrict__ out, float* __restrict__ alpha) {
   const float top = part ? obman_wave_max(part[threadIdx.x & (ROW_MAX_BLOCKS - 1)]) : weight_max(target, wide, ignore, rows, g_loss, 0, 1);
   int e = 0;
@@ -935,7 +944,7 @@ __global__ __launch_bounds__(1024) void rows_kernel(const float* __restrict__ ls
   if (r >= rows) return;
   const long t = target_of(target, wide, r);
   const float w = t == ignore ? 0.f : g_loss[r] * down * g_scale;
-  out[r] = RowConst{w == 0.f ? INFINITY : lse[r] * LOG2E - log2f(fabsf(w)), w, w == 0.f || t < 0 || t > 0x7fffffffL ? -1 : (int)t, 0};
+  out[r] = w == 0.f ? NO_ROW : row_const(lse[r].x, lse[r].y, w, t < 0 || t > 0x7fffffffL ? -1 : (int)t);
 }
 
 // The end of a piece: the slabs' sums times alpha in the gradient's own type (x: grid row 0, w: 1), and the bias gradient from the
@@ -1002,12 +1011,13 @@ struct Carve {  // scratch: offsets first, pointers once a base is there
 
 constexpr long PIECE_BYTES = 512L << 20;  // of g at a time
 
-// what the forward pass leaves for the backward pass: both operands in blocks, their scales, and per row the log-sum-exp and, if all
-// rows weigh the same, the constants
+// what the forward pass leaves for the backward pass: both operands in blocks, their scales, and per row the statistics (maximum, log2 of
+// the sum) and, if all rows weigh the same, the constants
 struct Keep {
   Side x, w;
   u16 *xp, *wp;
-  float *scales, *lse, *norm;
+  float *scales, *norm;
+  float2* lse;
   RowConst* rows;
   int ld;  // the width, up to whole blocks
   size_t bytes;
@@ -1029,7 +1039,7 @@ static Keep keep_of(const obman_class_loss_params& p, void* mem) {
   const long xr = up(p.rows, wide_of(p) ? BJ : BI), wr = up(p.classes, BI);  // (x has the rows of g)
   k.scales = c.take<float>(4);
   k.norm = k.scales + 2;
-  k.lse = c.take<float>(p.rows);
+  k.lse = c.take<float2>(p.rows);
   k.rows = c.take<RowConst>(p.reduction ? p.rows : 0);
   k.xp = c.take<u16>(xr * k.ld * planes);
   k.wp = c.take<u16>(wr * k.ld * planes);
@@ -1055,7 +1065,7 @@ constexpr int FEW_BLOCKS = 512;
 constexpr size_t FEW_LDS = 128 * 1024;  // of x: 32 rows of 4 KB, 64 of 2 KB
 struct Few {
   float2* part;
-  float *picked, *lse, *norm;
+  float *picked, *norm;
   int blocks, groups;
   size_t bytes, lds;
 };
@@ -1066,7 +1076,6 @@ static bool few_of(const obman_class_loss_params& p, void* mem, Few* o) {
   o->blocks = (int)(tiles < FEW_BLOCKS ? tiles : FEW_BLOCKS);
   o->part = c.take<float2>((size_t)o->blocks * FEW);
   o->picked = c.take<float>(FEW);
-  o->lse = c.take<float>(FEW);
   o->norm = c.take<float>(1);
   o->bytes = c.at;
   const int e = p.type == F32 ? 4 : 8;
@@ -1085,7 +1094,7 @@ template <int TYPE>
 static int few(const obman_class_loss_params& p, const Few& o, float* loss, hipStream_t st) {
   const int e = o.groups == 1 ? launch_few<TYPE, 1>(p, o, st) : launch_few<TYPE, 2>(p, o, st);
   if (e) return e;
-  few_join_kernel<<<1, 1024, 0, st>>>(o.part, o.blocks, (int)p.rows, p.classes, o.picked, p.target, p.target_wide, p.ignore_index, p.reduction, loss, o.lse, o.norm);
+  few_join_kernel<<<1, 1024, 0, st>>>(o.part, o.blocks, (int)p.rows, p.classes, o.picked, p.target, p.target_wide, p.ignore_index, p.reduction, loss, o.norm);
   OBMAN_LAUNCH_CHECK();
   return 0;
 }
