@@ -300,7 +300,8 @@ int obman_bf16_shadow(const float* src, uint16_t* dst, long n, obman_stream_t st
  * Forward: loss (rows floats, or one).  keep holds what the backward pass needs - it does not read x and w again; NULL (keeps = 0
  * for the sizes): none will follow, and up to 32 rows of 4 KB or 64 rows of 2 KB are then scored with one read of w as it is.
  * Backward: g_loss (rows floats, or one); dx, dw, db of the inputs' type, each may be NULL (need_* = 0 for the sizes).  The gradient
- * of the logits exists for a piece of the classes at a time, in the scratch.  Fixed summation order: the same bits every call.
+ * of the logits exists for a piece of the classes at a time, in the scratch; for 16-bit types it is rounded to their type, for fp32 it has
+ * 22 bits, and it ends at 2^-39 (fp16) or 2^-51 (fp32) of the largest row's weight.  Fixed summation order: the same bits every call.
  * obman_class_loss_sizes: bytes of keep and of the two calls' scratch ws, 256-byte aligned device memory. */
 typedef struct obman_class_loss_params {
   const void *x, *w, *bias, *target;

@@ -12,7 +12,9 @@
 // is written as hi + lo, two fp16 numbers (22 bits) after a power-of-two scaling of the whole tensor to 2^13 .. 2^14, and a product is
 // lo*hi + hi*lo + hi*hi: 2^-22 relative, an element 2^27 below the tensor's largest still has 11 bits, and three fp16 products are
 // 5 times the rate of the fp32 matrix instruction.  g has |g| <= max |c|: in fp16 it is scaled to 2^14.  Rounding g to 16 bits (its own
-// size, before sums of many rows or classes) costs as much again as rounding the result.
+// size, before sums of many rows or classes) costs as much again as rounding the result.  With fp32 operands g is hi + lo too, and its lo
+// is kept 2^12 times as large (the factor comes out of the other operand's hi): g is mostly probabilities, whose small ones are what a class
+// that is never a label learns from, and so its bits end at 2^-51 of max |c| instead of 2^-39.
 //
 // Rows that are ignored take no part: their x (which may be garbage) is packed as zeros, their g is zero.
 #include "common.h"
@@ -51,6 +53,7 @@ constexpr int BIAS_AT = STAGES * STAGE_BYTES, LDS_BYTES = BIAS_AT + BI * 4;
 constexpr long MOST_ROWS = 1L << 22;  // of an operand: sixteen blocks of its columns stay within 32-bit offsets
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float G_SCALE = 16384.f;  // |g| / max|c| <= 1 in fp16
+constexpr float G_LO = 4096.f;      // factor on g's lo: at 2^14 it is at most 2^2, and fp16 ends at 2^16
 
 template <bool SPLIT>
 constexpr int Step = SPLIT ? 16 : 32;  // columns of a block, and the contraction of a step
@@ -402,7 +405,7 @@ struct Grad {
               const float x = acc[fi][fj][(q + u) * 4 + e * 2], y = acc[fi][fj][(q + u) * 4 + e * 2 + 1];
               const u16 hx = narrow<T>(x), hy = narrow<T>(y);
               hi[u][e] = hx | (unsigned)hy << 16;
-              if constexpr (SPLIT) lo[u][e] = narrow<T>(x - widen<T>(hx)) | (unsigned)narrow<T>(y - widen<T>(hy)) << 16;
+              if constexpr (SPLIT) lo[u][e] = narrow<T>((x - widen<T>(hx)) * G_LO) | (unsigned)narrow<T>((y - widen<T>(hy)) * G_LO) << 16;
             }
           u16* to = o + (SPLIT ? (fi * 2 + q / 2) * rows_padded * 32 : fi * rows_padded * 32 + q * 8);
           {
@@ -495,7 +498,10 @@ struct SlabStore {
 // (1055); the matrix pipe is busy 56 - 57 % of cycles whose clock the chip holds at 1.6 - 1.75 GHz.  (Taking a fifth of the cycles out of
 // the forward product, by the blocked operands, the epilogue and the order of reads and loads, took 6 % off its time.)  fp32 at
 // 19 200 x 16 050 x 512: 70 % at 1.5 - 1.7 GHz, 1080 - 1220 Tflop/s of fp16 products.  A library's large bf16 product reaches 1375 here.
-template <bool A_KR, bool B_KR, int T, bool SPLIT, class Epi>
+// G: which operand is g (its lo is G_LO times as large)
+enum { G_NONE, G_A, G_B };
+__device__ __forceinline__ u32x4 lowered(u32x4 hi) { return __builtin_bit_cast(u32x4, __builtin_bit_cast(f16x8, hi) * (_Float16)(1.f / G_LO)); }
+template <bool A_KR, bool B_KR, int T, bool SPLIT, int G, class Epi>
 __device__ __forceinline__ void gemm(const Gemm& g, const Epi& epi, int id, char* smem) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int bi, bj, part;
@@ -557,7 +563,15 @@ __device__ __forceinline__ void gemm(const Gemm& g, const Epi& epi, int id, char
     products(a[0], b[0]);
     if (s + 2 < steps) issue();  // (here rather than before the reads: 2 - 5 % of the logits products)
     if constexpr (SPLIT) {
+      if constexpr (G == G_B) {
+#pragma unroll
+        for (int f = 0; f < 4; ++f) a[0][f] = lowered(a[0][f]);
+      }
       products(a[0], b[1]);
+      if constexpr (G == G_A) {
+#pragma unroll
+        for (int f = 0; f < 2; ++f) b[0][f] = lowered(b[0][f]);
+      }
       products(a[1], b[0]);
     } else {
       products(a[1], b[1]);
@@ -570,7 +584,7 @@ __device__ __forceinline__ void gemm(const Gemm& g, const Epi& epi, int id, char
 template <int T, bool SPLIT, class Epi>
 __global__ __launch_bounds__(WAVES * 64, 2) void logits_kernel(Gemm g, Epi epi) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  gemm<false, false, T, SPLIT>(g, epi, blockIdx.x, smem);
+  gemm<false, false, T, SPLIT, G_NONE>(g, epi, blockIdx.x, smem);
 }
 
 // dx and dw of a piece of the classes in one launch (each may have no blocks): both read the same g, and their blocks fill each
@@ -583,8 +597,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void grads_kernel(Gemm gx, Slab ex, 
   const bool is_x = ((int)blockIdx.x < first) == (x_first != 0);
   const int id = (int)blockIdx.x < first ? blockIdx.x : blockIdx.x - first;
   if (id >= (is_x ? nx : nw)) return;
-  if (is_x) gemm<WIDE, !WIDE, T, SPLIT>(gx, SlabStore<WIDE>{ex}, id, smem);
-  else gemm<true, true, T, SPLIT>(gw, SlabStore<WIDE>{ew}, id, smem);
+  if (is_x) gemm<WIDE, !WIDE, T, SPLIT, WIDE ? G_B : G_A>(gx, SlabStore<WIDE>{ex}, id, smem);
+  else gemm<true, true, T, SPLIT, WIDE ? G_B : G_A>(gw, SlabStore<WIDE>{ew}, id, smem);
 }
 
 // ------------------------------------------------------------------------------------------------------- operands and rows

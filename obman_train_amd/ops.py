@@ -997,8 +997,10 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
     ``ignore_index`` has loss 0 and gradient 0 and takes no part in any gradient, even if its features are not finite; if every row
     is ignored the mean is 0.  A target that is neither a class nor ``ignore_index`` makes the loss NaN.  A bias of -inf takes a class
     out of the sum.  Gradients for ``x``, ``weight`` and ``bias`` (only those that need one are computed), once differentiable;
-    summation orders are fixed, so the same call gives the same bits.  With ``"none"`` in fp16 and fp32, rows whose gradient is less than
-    about 2^-16 of the largest row's are exact relative to that one, not to themselves.  Rows and classes up to 2^22, width up to 16384."""
+    summation orders are fixed, so the same call gives the same bits.  The logits' gradient, of which dx and dw are sums, is rounded to 16-bit
+    inputs' own type first (8 bits in bf16, 11 in fp16; db is summed before); in fp32 it has 22 bits.  In fp16 and fp32 it ends at 2^-39 and
+    2^-51 of the largest row's weight (the loss's gradient, with ``"none"`` its largest entry): smaller probabilities give no gradient.  Rows
+    and classes up to 2^22, width up to 16384."""
     if reduction not in _REDUCTIONS:
         raise ValueError("reduction must be 'none', 'sum' or 'mean', got %r" % (reduction,))
     for name, t in (("x", x), ("weight", weight), ("target", target), ("bias", bias)):
