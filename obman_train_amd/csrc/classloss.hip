@@ -10,8 +10,11 @@
 //
 // All products run on 16-bit matrix instructions with fp32 accumulators.  bf16 and fp16 operands go in as they are.  An fp32 operand
 // is written as hi + lo, two fp16 numbers (22 bits) after a power-of-two scaling of the whole tensor to 2^13 .. 2^14, and a product is
-// lo*hi + hi*lo + hi*hi: 2^-22 relative, an element 2^27 below the tensor's largest still has 11 bits, and three fp16 products are
-// 5 times the rate of the fp32 matrix instruction.  g has |g| <= max |c|: in fp16 it is scaled to 2^14.  Rounding g to 16 bits (its own
+// lo*hi + hi*lo + hi*hi: 2^-22 relative, and three fp16 products are 5 times the rate of the fp32 matrix instruction.  One scale for the
+// whole tensor ends at 2^-39 of its largest element, so this holds while every row's largest element (all zeros aside) is within
+// SPREAD = 2^16 of it: 2^-22 of the row's own.  The pass that finds the largest element finds that out too, on the device; if a row of x or
+// a class of w lies further off, the same kernels take the operands as fp32 and the fp32 instruction (FULL below; 19 200 x 16 050 x 512 forward and
+// backward: 9.6 ms against 3.7).  g has |g| <= max |c|: in fp16 it is scaled to 2^14.  Rounding g to 16 bits (its own
 // size, before sums of many rows or classes) costs as much again as rounding the result.  With fp32 operands g is hi + lo too, and its lo
 // is kept 2^12 times as large (the factor comes out of the other operand's hi): g is mostly probabilities, whose small ones are what a class
 // that is never a label learns from, and so its bits end at 2^-51 of max |c| instead of 2^-39.
@@ -53,10 +56,12 @@ constexpr int BIAS_AT = STAGES * STAGE_BYTES, LDS_BYTES = BIAS_AT + BI * 4;
 constexpr long MOST_ROWS = 1L << 22;  // of an operand: sixteen blocks of its columns stay within 32-bit offsets
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float G_SCALE = 16384.f;  // |g| / max|c| <= 1 in fp16
+constexpr float SPREAD = 65536.f;
 constexpr float G_LO = 4096.f;      // factor on g's lo: at 2^14 it is at most 2^2, and fp16 ends at 2^16
 
 template <bool SPLIT>
 constexpr int Step = SPLIT ? 16 : 32;  // columns of a block, and the contraction of a step
+// FULL: the block's 64 bytes are 16 fp32 numbers instead of 16 hi beside 16 lo.  Places, tiles and loads are the same.
 
 struct Side {  // [blocks][rows][32]
   const u16* p;
@@ -69,6 +74,7 @@ struct Gemm {
   long k_part;      // of it per part
   int ti, tj, parts; // tiles, and parts of the contraction
   int na, nb;       // column blocks of a / b (an operand whose rows are contracted: tiles that run over its columns repeat the last block)
+  const float* full; // fp32 operands: not 0 where they are kept in full
 };
 
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, unsigned lds, unsigned voff) {
@@ -114,8 +120,9 @@ struct Operand {
   }
 };
 
-// fragment of 32 rows x 16 k: lane -> row lane % 32, k = 8 (lane / 32) .. + 7; of the step's two halves, or of hi and lo
-template <bool KR, bool SPLIT>
+// fragment of 32 rows x 16 k: lane -> row lane % 32, k = 8 (lane / 32) .. + 7; of the step's two halves, or of hi and lo.  FULL: of 8 k,
+// lane -> k = 4 (lane / 32) .. + 3
+template <bool KR, bool SPLIT, bool FULL>
 struct Frag {
   unsigned off[2];
   __device__ __forceinline__ void init(int first_row, int lane) {  // first_row: a multiple of 32
@@ -124,6 +131,7 @@ struct Frag {
       // the transposing read: in a group of 16 lanes, lane c receives element c of the four rows that lanes 4 r .. 4 r + 3 point at
       const int k = 8 * (lane >> 5) + ((lane & 15) >> 2), right = (lane >> 4) & 1;
       if constexpr (!KR) off[h] = (first_row + (lane & 31)) * 64 + ((2 * h + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16;
+      else if constexpr (FULL) off[h] = first_row * 64 + right * 1024 + (8 * h + 4 * (lane >> 5)) * 64 + (((lane & 15) >> 2) ^ (right << 1)) * 16 + (lane & 3) * 4;
       else if constexpr (!SPLIT) off[h] = first_row * 64 + (h * 16 + k) * 64 + right * 32 + (lane & 3) * 8;
       else off[h] = first_row * 64 + right * 1024 + k * 64 + (h ^ right) * 32 + (lane & 3) * 8;
     }
@@ -131,6 +139,12 @@ struct Frag {
   __device__ __forceinline__ u32x4 read(const char* tile, int f, int h) const {
     const char* p = tile + off[h] + f * 2048;
     if constexpr (!KR) return *reinterpret_cast<const u32x4*>(p);
+    if constexpr (KR && FULL) {  // (two lanes a bank: this path is for the rare tensor)
+      u32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const unsigned*>(p + e * 64);
+      return v;
+    }
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p));
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p + 4 * 64));
     return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -141,6 +155,12 @@ template <int T>
 __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
   if constexpr (T == BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ f32x16 mfma_f32(u32x4 a, u32x4 b, f32x16 c) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+  return c;
 }
 
 template <int T>
@@ -296,6 +316,7 @@ struct Stats {
   float2* part;  // [ti][rows]
   float* picked; // [rows]
   __device__ __forceinline__ void before(const Gemm&, const Ctx& c, f32x16 (&acc)[4][2]) const { bias.before(c, acc); }
+  template <bool FULL>
   __device__ __forceinline__ void after(const Gemm& g, const Ctx& c, f32x16 (&acc)[4][2]) const {
     float2* red = reinterpret_cast<float2*>(c.smem);
     bias.finish(c, acc);
@@ -359,6 +380,7 @@ struct Grad {
   int columns;      // of out
   float* sums;      // [tj][columns]: the bias gradient's parts, summed before g is rounded
   __device__ __forceinline__ void before(const Gemm&, const Ctx& c, f32x16 (&acc)[4][2]) const { bias.before(c, acc); }
+  template <bool FULL>
   __device__ __forceinline__ void after(const Gemm& g, const Ctx& c, f32x16 (&acc)[4][2]) const {
     bias.finish(c, acc);
 #pragma unroll
@@ -395,6 +417,13 @@ struct Grad {
 #pragma unroll
       for (int fi = 0; fi < 4; ++fi) {
         if (c.i0 + c.wi * 128 + fi * 32 >= columns) continue;
+        if constexpr (FULL) {  // four classes a lane, 16 bytes as they are
+          float* f = reinterpret_cast<float*>(out) + ((c.i0 + c.wi * 128 + fi * 32) / Step<SPLIT> * rows_padded + r) * 16 + 4 * (c.lane >> 5);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<f32x4*>(f + (q >> 1) * rows_padded * 16 + (q & 1) * 8) = f32x4{acc[fi][fj][q * 4], acc[fi][fj][q * 4 + 1], acc[fi][fj][q * 4 + 2], acc[fi][fj][q * 4 + 3]};
+          continue;
+        }
 #pragma unroll
         for (int q = 0; q < 4; q += 2) {
           unsigned hi[2][2], lo[2][2];
@@ -454,6 +483,7 @@ template <bool WIDE>
 struct SlabStore {
   Slab s;
   __device__ __forceinline__ void before(const Gemm&, const Ctx&, f32x16 (&acc)[4][2]) const { clear(acc); }
+  template <bool FULL>
   __device__ __forceinline__ void after(const Gemm& g, const Ctx& c, f32x16 (&acc)[4][2]) const {
     float* o = s.out + c.split * s.slab;
     const int ld = s.ld;
@@ -501,8 +531,8 @@ struct SlabStore {
 // G: which operand is g (its lo is G_LO times as large)
 enum { G_NONE, G_A, G_B };
 __device__ __forceinline__ u32x4 lowered(u32x4 hi) { return __builtin_bit_cast(u32x4, __builtin_bit_cast(f16x8, hi) * (_Float16)(1.f / G_LO)); }
-template <bool A_KR, bool B_KR, int T, bool SPLIT, int G, class Epi>
-__device__ __forceinline__ void gemm(const Gemm& g, const Epi& epi, int id, char* smem) {
+template <bool A_KR, bool B_KR, int T, bool SPLIT, bool FULL, int G, class Epi>
+__device__ __forceinline__ void gemm_as(const Gemm& g, const Epi& epi, int id, char* smem) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int bi, bj, part;
   tile_of(g, id, bi, bj, part);
@@ -515,8 +545,8 @@ __device__ __forceinline__ void gemm(const Gemm& g, const Epi& epi, int id, char
   Operand<B_KR, BJ, SPLIT> ob;
   oa.init(g.a, bi * (BI / K), g.na, wave, lane);
   ob.init(g.b, bj * (BJ / K), g.nb, wave, lane);
-  Frag<A_KR, SPLIT> fa;
-  Frag<B_KR, SPLIT> fb;
+  Frag<A_KR, SPLIT, FULL> fa;
+  Frag<B_KR, SPLIT, FULL> fb;
   fa.init(ctx.wi * 128, lane);
   fb.init(ctx.wj * 64, lane);
   const long kb = part * g.k_part, ke = kb + g.k_part < g.k ? kb + g.k_part : g.k;
@@ -540,7 +570,7 @@ __device__ __forceinline__ void gemm(const Gemm& g, const Epi& epi, int id, char
 #pragma unroll
     for (int f = 0; f < 4; ++f)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) acc[f][h] = mfma<T>(a[f], b[h], acc[f][h]);
+      for (int h = 0; h < 2; ++h) acc[f][h] = FULL ? mfma_f32(a[f], b[h], acc[f][h]) : mfma<T>(a[f], b[h], acc[f][h]);
     __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -562,7 +592,7 @@ __device__ __forceinline__ void gemm(const Gemm& g, const Epi& epi, int id, char
     from = from == smem + (STAGES - 1) * STAGE_BYTES ? smem : from + STAGE_BYTES;
     products(a[0], b[0]);
     if (s + 2 < steps) issue();  // (here rather than before the reads: 2 - 5 % of the logits products)
-    if constexpr (SPLIT) {
+    if constexpr (SPLIT && !FULL) {
       if constexpr (G == G_B) {
 #pragma unroll
         for (int f = 0; f < 4; ++f) a[0][f] = lowered(a[0][f]);
@@ -578,7 +608,17 @@ __device__ __forceinline__ void gemm(const Gemm& g, const Epi& epi, int id, char
     }
   }
   __syncthreads();
-  epi.after(g, ctx, acc);
+  epi.template after<FULL>(g, ctx, acc);
+}
+template <bool A_KR, bool B_KR, int T, bool SPLIT, int G, class Epi>
+__device__ __forceinline__ void gemm(const Gemm& g, const Epi& epi, int id, char* smem) {
+  if constexpr (SPLIT) {
+    if (*g.full != 0.f) {
+      gemm_as<A_KR, B_KR, T, SPLIT, true, G>(g, epi, id, smem);
+      return;
+    }
+  }
+  gemm_as<A_KR, B_KR, T, SPLIT, false, G>(g, epi, id, smem);
 }
 
 template <int T, bool SPLIT, class Epi>
@@ -603,59 +643,98 @@ __global__ __launch_bounds__(WAVES * 64, 2) void grads_kernel(Gemm gx, Slab ex, 
 
 // ------------------------------------------------------------------------------------------------------- operands and rows
 
-// largest finite |x| of the kept rows of x (grid row 0) and of w (1): MAX_PARTS block maxima each
+// of the kept rows of x (grid row 0) and of w (1): the largest finite |element|, and the least of the rows' largest (rows of zeros
+// aside).  MAX_PARTS block values each: [largest of x, of w, least of x, of w]
 constexpr int MAX_PARTS = 512;
+__device__ __forceinline__ float wave_max(float m) {  // within 16 lanes, then of the four 16s: a tenth of the time of six shuffles
+  m = fmaxf(m, obman_dpp<0xB1>(m));
+  m = fmaxf(m, obman_dpp<0x4E>(m));
+  m = fmaxf(m, obman_dpp<0x141>(m));
+  m = fmaxf(m, obman_dpp<0x140>(m));
+  u32x2 s = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+  m = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+  s = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
 __global__ __launch_bounds__(256) void absmax_kernel(const float* __restrict__ x, long rows, const float* __restrict__ w, long classes, int width, const void* target, int wide,
                                                     long ignore, float* __restrict__ part) {
   const bool first = blockIdx.y == 0;
   const float* p = first ? x : w;
   const long n = first ? rows : classes;
   const int lane = threadIdx.x & 63, full = width & ~3;
-  float m = 0.f;
+  float top = 0.f, least = INFINITY;
   for (long r = (long)blockIdx.x * 4 + (threadIdx.x >> 6); r < n; r += MAX_PARTS * 4) {  // a wave takes a row
     if (first && target_of(target, wide, r) == ignore) continue;
     const float* q = p + r * width;
+    float m = 0.f;
     for (int i = lane * 4; i < full; i += 256) {
       const f32x4u v = *reinterpret_cast<const f32x4u*>(q + i);
 #pragma unroll
       for (int e = 0; e < 4; ++e) { const float a = fabsf(v[e]); m = a > m && a < INFINITY ? a : m; }
     }
     if (full + lane < width) { const float a = fabsf(q[full + lane]); m = a > m && a < INFINITY ? a : m; }
+    m = wave_max(m);
+    top = fmaxf(top, m);
+    if (m > 0.f) least = fminf(least, m);
   }
-  m = obman_wave_max(m);
-  __shared__ float red[4];
-  if (lane == 0) red[threadIdx.x >> 6] = m;
+  __shared__ float red[2][4];
+  if (lane == 0) { red[0][threadIdx.x >> 6] = top; red[1][threadIdx.x >> 6] = least; }
   __syncthreads();
-  if (threadIdx.x == 0) part[blockIdx.y * MAX_PARTS + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  if (threadIdx.x == 0) {
+    part[blockIdx.y * MAX_PARTS + blockIdx.x] = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    part[(2 + blockIdx.y) * MAX_PARTS + blockIdx.x] = fminf(fminf(red[1][0], red[1][1]), fminf(red[1][2], red[1][3]));
+  }
 }
 
-// the power of two that brings the largest element to 2^13 .. 2^14 (1 for an all-zero tensor); every thread of the block has it
-__device__ float scale_of(const float* __restrict__ part) {
-  __shared__ float red[4];
-  float m = fmaxf(part[threadIdx.x], part[threadIdx.x + 256]);
-  m = obman_wave_max(m);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+// Every thread of the block: whether fp32 operands are kept in full, and the powers of two that bring the largest elements to 2^13 .. 2^14
+// (1 for an all-zero tensor, and in full)
+struct Scales { float scale[2]; bool full; };
+__device__ Scales scales_of(const float* __restrict__ part) {
+  __shared__ float red[4][4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float* p = part + k * MAX_PARTS + threadIdx.x;
+    const float m = k < 2 ? wave_max(fmaxf(p[0], p[256])) : -wave_max(-fminf(p[0], p[256]));
+    if (lane == 0) red[k][wave] = m;
+  }
   __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  int e = 0;
-  if (m > 0.f) (void)frexpf(m, &e);  // m = f 2^e, f in [0.5, 1)
-  e = 14 - e;
-  e = e > 120 ? 120 : e < -112 ? -112 : e;  // a power of two and its inverse are normal numbers
-  return m > 0.f ? ldexpf(1.f, e) : 1.f;
+  Scales o;
+  o.full = false;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float m = fmaxf(fmaxf(red[k][0], red[k][1]), fmaxf(red[k][2], red[k][3]));
+    const float least = fminf(fminf(red[2 + k][0], red[2 + k][1]), fminf(red[2 + k][2], red[2 + k][3]));
+    int e = 0;
+    if (m > 0.f) (void)frexpf(m, &e);  // m = f 2^e, f in [0.5, 1)
+    e = 14 - e;
+    e = e > 120 ? 120 : e < -112 ? -112 : e;  // a power of two and its inverse are normal numbers
+    o.scale[k] = m > 0.f ? ldexpf(1.f, e) : 1.f;
+    o.full |= m > 0.f && m * (1.f / SPREAD) > least;
+  }
+  if (o.full) o.scale[0] = o.scale[1] = 1.f;
+  return o;
 }
 
 // x (grid row 0) and w (1) into blocks of columns, [blocks][padded rows][32]: zeros behind the width, behind the last row and for
 // ignored rows
 struct Pack { const void* src; u16* dst; long rows, padded; };
+constexpr int FULL_AT = 3;  // where the scales say whether the operands are kept in full
 template <int TYPE>
 __global__ __launch_bounds__(256) void pack_kernel(Pack px, Pack pw, int width, int chunks, const void* target, int wide, long ignore, const float* __restrict__ part,
                                                   float* __restrict__ scale) {
   const bool first = blockIdx.y == 0;
   const Pack p = first ? px : pw;
   float sc = 1.f;
+  bool full = false;
   if constexpr (TYPE == F32) {
-    sc = scale_of(part + blockIdx.y * MAX_PARTS);
-    if (blockIdx.x == 0 && threadIdx.x == 0) scale[blockIdx.y] = sc;
+    const Scales s = scales_of(part);
+    sc = s.scale[blockIdx.y];
+    full = s.full;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      scale[blockIdx.y] = sc;
+      if (first) scale[FULL_AT] = full ? 1.f : 0.f;
+    }
   }
   const long n = p.padded * chunks;  // of 8 columns
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
@@ -677,6 +756,13 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack px, Pack pw, int width, 
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = c + e < width ? q[e] : 0.f;
         }
+        if (full) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {  // the eight in a row, two 16-bit halves each
+            hi[2 * e] = (u16)(__float_as_uint(v[e]) & 0xffffu), hi[2 * e + 1] = (u16)(__float_as_uint(v[e]) >> 16);
+            lo[2 * e] = (u16)(__float_as_uint(v[e + 4]) & 0xffffu), lo[2 * e + 1] = (u16)(__float_as_uint(v[e + 4]) >> 16);
+          }
+        } else
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float y = v[e] * sc;
@@ -696,9 +782,9 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack px, Pack pw, int width, 
       }
     }
     constexpr int K = Step<TYPE == F32>;
-    u16* o = p.dst + ((long)(c / K) * p.padded + r) * 32 + c % K;
+    u16* o = p.dst + ((long)(c / K) * p.padded + r) * 32 + (full ? 2 : 1) * (c % K);
     *reinterpret_cast<u32x4*>(o) = *reinterpret_cast<u32x4*>(hi);
-    if constexpr (TYPE == F32) *reinterpret_cast<u32x4*>(o + 16) = *reinterpret_cast<u32x4*>(lo);
+    if constexpr (TYPE == F32) *reinterpret_cast<u32x4*>(o + (full ? 8 : 16)) = *reinterpret_cast<u32x4*>(lo);
   }
 }
 
@@ -770,10 +856,8 @@ __global__ __launch_bounds__(256) void few_kernel(const void* __restrict__ xs, c
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const u32x4 b = *reinterpret_cast<const u32x4*>(xl + (p * 2 * R + g * 32) * 16);
-        if constexpr (TYPE == F32) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[g] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(w[e]), __uint_as_float(b[e]), acc[g], 0, 0, 0);
-        } else acc[g] = mfma<TYPE>(w, b, acc[g]);
+        if constexpr (TYPE == F32) acc[g] = mfma_f32(w, b, acc[g]);
+        else acc[g] = mfma<TYPE>(w, b, acc[g]);
       }
     };
     int p = 0;
@@ -861,11 +945,18 @@ __global__ __launch_bounds__(1024) void few_join_kernel(const float2* __restrict
   total_loss(l, k, reduction == 2, loss, norm);
 }
 
+// what g is scaled by: to use fp16's range, and not at all where it is kept in fp32
+struct GScale {
+  float value;
+  const float* full;
+  __device__ __forceinline__ float get() const { return full && *full != 0.f ? 1.f : value; }
+};
+
 // Per row: join over the tiles of classes; loss per row, what the backward pass needs of the row if every row weighs the same, and per
 // block of 64 rows the sum of losses and the number of kept rows.  WHOLE: one block does all rows and the reduction.
 template <bool WHOLE>
 __global__ __launch_bounds__(WHOLE ? 1024 : 256) void join_rows_kernel(const float2* __restrict__ part, int tiles, long rows, long classes, const float* __restrict__ picked,
-                                                                      const void* target, int wide, long ignore, int reduction, float g_scale, float2* __restrict__ lse,
+                                                                      const void* target, int wide, long ignore, int reduction, GScale g_scale, float2* __restrict__ lse,
                                                                       float* __restrict__ loss, RowConst* __restrict__ consts, double2* __restrict__ sums, float* __restrict__ norm) {
   constexpr int GROUPS = WHOLE ? 4 : 1;  // of 64 rows x 4 threads
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave & 3, group = wave >> 2;
@@ -888,7 +979,7 @@ __global__ __launch_bounds__(WHOLE ? 1024 : 256) void join_rows_kernel(const flo
       lse[r] = make_float2(m, log_s);
       const float row = row_loss(m, log_s, t, classes, ignore, picked, r);
       if (reduction == 0) loss[r] = row;
-      if (consts) consts[r] = none ? NO_ROW : row_const(m, log_s, g_scale, outside ? -1 : (int)t);
+      if (consts) consts[r] = none ? NO_ROW : row_const(m, log_s, g_scale.get(), outside ? -1 : (int)t);
       l += row;
       kept += t != ignore;
     }
@@ -947,7 +1038,7 @@ __global__ __launch_bounds__(1024) void row_max_kernel(const void* target, int w
 // A gradient for every row: RowConst with its weight, scaled to at most 1 in magnitude by a power of two; alpha takes it back.  part: the
 // ROW_MAX_BLOCKS maxima of row_max_kernel, or NULL: every block looks through all rows.
 __global__ __launch_bounds__(1024) void rows_kernel(const float2* __restrict__ lse, const void* target, int wide, long ignore, long rows, const float* __restrict__ g_loss,
-                                                   const float* __restrict__ part, float g_scale, RowConst* __restrict__ out, float* __restrict__ alpha) {
+                                                   const float* __restrict__ part, GScale g_scale, RowConst* __restrict__ out, float* __restrict__ alpha) {
   const float top = part ? obman_wave_max(part[threadIdx.x & (ROW_MAX_BLOCKS - 1)]) : weight_max(target, wide, ignore, rows, g_loss, 0, 1);
   int e = 0;
   if (top > 0.f) (void)frexpf(top, &e);
@@ -957,18 +1048,18 @@ __global__ __launch_bounds__(1024) void rows_kernel(const float2* __restrict__ l
   const long r = (long)blockIdx.x * 1024 + threadIdx.x;
   if (r >= rows) return;
   const long t = target_of(target, wide, r);
-  const float w = t == ignore ? 0.f : g_loss[r] * down * g_scale;
+  const float w = t == ignore ? 0.f : g_loss[r] * down * g_scale.get();
   out[r] = w == 0.f ? NO_ROW : row_const(lse[r].x, lse[r].y, w, t < 0 || t > 0x7fffffffL ? -1 : (int)t);
 }
 
 // The end of a piece: the slabs' sums times alpha in the gradient's own type (x: grid row 0, w: 1), and the bias gradient from the
-// column sums of the tiles of rows, in order (2).  rows = 0: nothing to do.  alpha = *alpha[0] * *alpha[1] / g_scale.
+// column sums of the tiles of rows, in order (2).  rows = 0: nothing to do.  alpha = *a * *b / g_scale.
 struct Finish { const float* slabs; int n; long slab, rows; const float* scale; void* out; };
 struct FinishBias { const float* sums; int n, columns; long classes; void* out; };
 struct Alpha {
   const float *a, *b;
-  float over;
-  __device__ __forceinline__ float value() const { return *a * (b ? *b : 1.f) * over; }
+  GScale g_scale;  // a power of two
+  __device__ __forceinline__ float value() const { return *a * (b ? *b : 1.f) / g_scale.get(); }
 };
 __global__ __launch_bounds__(256) void finish_kernel(Finish fx, Finish fw, FinishBias fb, int ld, int width, Alpha alpha, int type) {
   if (blockIdx.y == 2) {
@@ -1025,7 +1116,7 @@ struct Carve {  // scratch: offsets first, pointers once a base is there
 
 constexpr long PIECE_BYTES = 512L << 20;  // of g at a time
 
-// what the forward pass leaves for the backward pass: both operands in blocks, their scales, and per row the statistics (maximum, log2 of
+// what the forward pass leaves for the backward pass: both operands in blocks, their scales and whether they are kept in full, and per row the statistics (maximum, log2 of
 // the sum) and, if all rows weigh the same, the constants
 struct Keep {
   Side x, w;
@@ -1126,7 +1217,7 @@ static Forward forward_of(const obman_class_loss_params& p, void* mem) {
   Forward o;
   o.ti = obman_cdiv(p.classes, BI);
   o.row_blocks = obman_cdiv(p.rows, 64);
-  o.max_part = c.take<float>(2 * MAX_PARTS);
+  o.max_part = c.take<float>(4 * MAX_PARTS);
   o.part = c.take<float2>((size_t)o.ti * p.rows);
   o.picked = c.take<float>(p.rows);
   o.sums = c.take<double2>(o.row_blocks);
@@ -1216,8 +1307,8 @@ static int blocks_for(long items) {
   return (int)(b < 1 ? 1 : b > 8192 ? 8192 : b);
 }
 
-static Gemm gemm_of(const Side& a, const Side& b, long ni, long nj, long k, int parts, int na, int nb) {
-  return Gemm{a, b, ni, nj, k, up((k + parts - 1) / parts, 32), obman_cdiv(ni, BI), obman_cdiv(nj, BJ), parts, na, nb};
+static Gemm gemm_of(const Keep& keep, const Side& a, const Side& b, long ni, long nj, long k, int parts, int na, int nb) {
+  return Gemm{a, b, ni, nj, k, up((k + parts - 1) / parts, 32), obman_cdiv(ni, BI), obman_cdiv(nj, BJ), parts, na, nb, keep.scales + FULL_AT};
 }
 template <int T, bool SPLIT, class Epi>
 static int launch_logits(const Gemm& g, const Epi& epi, hipStream_t st) {
@@ -1253,12 +1344,12 @@ static int check(const obman_class_loss_params* p) {
 }
 
 // |g| in 16 bits: scaled in fp16
-static float g_scale_of(int type) { return type == BF16 ? 1.f : G_SCALE; }
+static GScale g_scale_of(int type, const Keep& k) { return GScale{type == BF16 ? 1.f : G_SCALE, type == F32 ? k.scales + FULL_AT : nullptr}; }
 
 template <int T, bool SPLIT>
 static int forward(const obman_class_loss_params& p, const Keep& k, const Forward& o, hipStream_t st) {
   const Stats<SPLIT> epi{{Scale{SPLIT ? k.scales : nullptr, SPLIT ? k.scales + 1 : nullptr}, p.bias, p.type, 0, p.classes}, p.target, p.target_wide, o.part, o.picked};
-  return launch_logits<T, SPLIT>(gemm_of(k.w, k.x, p.classes, p.rows, k.ld, 1, 0, 0), epi, st);
+  return launch_logits<T, SPLIT>(gemm_of(k, k.w, k.x, p.classes, p.rows, k.ld, 1, 0, 0), epi, st);
 }
 
 template <int T, bool SPLIT, bool WIDE>
@@ -1273,10 +1364,10 @@ static int backward(const obman_class_loss_params& p, const Keep& k, const Backw
     const bool last = v0 + nv == p.classes;
     const Side w{k.wp + v0 * 32, k.w.rows}, gs{o.g, xr};
     const Grad<T, SPLIT> ge{{Scale{sx, sw}, p.bias, p.type, v0, v0 + nv}, rows, p.rows, xr, o.g, (int)kv, db ? o.sums : nullptr};
-    if (const int e = launch_logits<T, SPLIT>(gemm_of(w, k.x, kv, xr, ld, 1, 0, 0), ge, st)) return e;
+    if (const int e = launch_logits<T, SPLIT>(gemm_of(k, w, k.x, kv, xr, ld, 1, 0, 0), ge, st)) return e;
     const int d = ld / Step<SPLIT>, v = (int)(kv / Step<SPLIT>);  // column blocks of the operands and of g
-    const Gemm gx = WIDE ? gemm_of(w, gs, ld, p.rows, kv, o.parts.x, d, 0) : gemm_of(gs, w, p.rows, ld, kv, o.parts.x, 0, d);
-    const Gemm gw = WIDE ? gemm_of(k.x, gs, ld, nv, xr, o.parts.w, d, v) : gemm_of(gs, k.x, nv, ld, xr, o.parts.w, v, d);
+    const Gemm gx = WIDE ? gemm_of(k, w, gs, ld, p.rows, kv, o.parts.x, d, 0) : gemm_of(k, gs, w, p.rows, ld, kv, o.parts.x, 0, d);
+    const Gemm gw = WIDE ? gemm_of(k, k.x, gs, ld, nv, xr, o.parts.w, d, v) : gemm_of(k, gs, k.x, nv, ld, xr, o.parts.w, v, d);
     const int nx = dx ? gx.ti * gx.tj * gx.parts : 0, nw = dw ? gw.ti * gw.tj * gw.parts : 0;
     if (nx + nw) {
       const int second = o.parts.x_first ? nw : nx, first = nx + nw - second;
@@ -1335,7 +1426,7 @@ int obman_class_loss_fwd(const obman_class_loss_params* p, void* keep, void* ws,
                             : cl::forward<cl::F16, false>(*p, k, o, st);
   if (e) return e;
   cl::RowConst* consts = keep && p->reduction ? k.rows : nullptr;
-  const float gs = cl::g_scale_of(p->type);
+  const cl::GScale gs = cl::g_scale_of(p->type, k);
   if (p->rows <= cl::WHOLE_ROWS && p->rows * o.ti <= cl::WHOLE_PARTS) {
     cl::join_rows_kernel<true><<<1, 1024, 0, st>>>(o.part, o.ti, p->rows, p->classes, o.picked, p->target, p->target_wide, p->ignore_index, p->reduction, gs, k.lse, loss,
                                                    consts, nullptr, k.norm);
@@ -1360,8 +1451,8 @@ int obman_class_loss_bwd(const obman_class_loss_params* p, const void* keep, con
   hipStream_t st = (hipStream_t)stream;
   const cl::Keep k = cl::keep_of(*p, const_cast<void*>(keep));
   const cl::Backward o = cl::backward_of(*p, k, ws, dx != nullptr, dw != nullptr, db != nullptr);
-  const float gs = cl::g_scale_of(p->type);
-  cl::Alpha alpha{g_loss, k.norm, 1.f / gs};
+  const cl::GScale gs = cl::g_scale_of(p->type, k);
+  cl::Alpha alpha{g_loss, k.norm, gs};
   if (!p->reduction) {
     const bool split = p->rows > cl::SCAN_ROWS;
     if (split) {
@@ -1371,7 +1462,7 @@ int obman_class_loss_bwd(const obman_class_loss_params* p, const void* keep, con
     cl::rows_kernel<<<obman_cdiv(p->rows, 1024), 1024, 0, st>>>(k.lse, p->target, p->target_wide, p->ignore_index, p->rows, g_loss, split ? o.row_max : nullptr, gs, o.rows,
                                                                 o.alpha);
     OBMAN_LAUNCH_CHECK();
-    alpha = cl::Alpha{o.alpha, nullptr, 1.f / gs};
+    alpha = cl::Alpha{o.alpha, nullptr, gs};
   }
   const cl::RowConst* rows = p->reduction ? k.rows : o.rows;
   if (cl::wide_of(*p))
