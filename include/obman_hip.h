@@ -298,7 +298,7 @@ int obman_bf16_shadow(const float* src, uint16_t* dst, long n, obman_stream_t st
  * An element of fp32 x or w is right to 2^-22 of its row's largest (pairs of fp16; the fp32 instruction where a row's largest element is
  * below 2^-16 of the tensor's, rows of zeros aside, which the device finds out).
  * reduction: 0 per row, 1 sum, 2 mean over the rows that are not ignored (0 if there are none).
- * rows, classes: at most 2^22; width: at most 16384.
+ * rows, classes: at most 2^22 each; width: at most 16384; the forward scratch takes 8 bytes for each row and 256 classes.
  * Forward: loss (rows floats, or one).  keep holds what the backward pass needs - it does not read x and w again; NULL (keeps = 0
  * for the sizes): none will follow, and up to 32 rows of 4 KB or 64 rows of 2 KB are then scored with one read of w as it is.
  * Backward: g_loss (rows floats, or one); dx, dw, db of the inputs' type, each may be NULL (need_* = 0 for the sizes).  The gradient

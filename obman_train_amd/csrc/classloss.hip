@@ -324,7 +324,7 @@ struct Stats {
 #pragma unroll
     for (int fj = 0; fj < 2; ++fj) {
       const long r = c.j0 + c.wj * 64 + fj * 32 + (c.lane & 31);
-      const int t = target_at(r < g.nj ? target_of(target, target_wide, r) : -1, c.i0 + c.wi * 128, c.lane);
+      const int t = target_at(r < g.nj ? target_of(target, target_wide, r) : -1, bias.class0 + c.i0 + c.wi * 128, c.lane);
       if (__any(t >= 0)) {
         float z = 0.f;
 #pragma unroll
@@ -1346,10 +1346,18 @@ static int check(const obman_class_loss_params* p) {
 // |g| in 16 bits: scaled in fp16
 static GScale g_scale_of(int type, const Keep& k) { return GScale{type == BF16 ? 1.f : G_SCALE, type == F32 ? k.scales + FULL_AT : nullptr}; }
 
+// Pieces of the classes again, but only for the launch: it may have fewer than 2^32 threads.
+constexpr long MOST_BLOCKS = 1L << 23;
 template <int T, bool SPLIT>
 static int forward(const obman_class_loss_params& p, const Keep& k, const Forward& o, hipStream_t st) {
-  const Stats<SPLIT> epi{{Scale{SPLIT ? k.scales : nullptr, SPLIT ? k.scales + 1 : nullptr}, p.bias, p.type, 0, p.classes}, p.target, p.target_wide, o.part, o.picked};
-  return launch_logits<T, SPLIT>(gemm_of(k, k.w, k.x, p.classes, p.rows, k.ld, 1, 0, 0), epi, st);
+  const long per = MOST_BLOCKS / obman_cdiv(p.rows, BJ);  // tiles of classes a launch: 256 for the most rows
+  for (long t0 = 0; t0 < o.ti; t0 += per) {
+    const long v0 = t0 * BI, nv = p.classes - v0 < per * BI ? p.classes - v0 : per * BI;
+    const Side w{k.wp + v0 * 32, k.w.rows};
+    const Stats<SPLIT> epi{{Scale{SPLIT ? k.scales : nullptr, SPLIT ? k.scales + 1 : nullptr}, p.bias, p.type, v0, p.classes}, p.target, p.target_wide, o.part + t0 * p.rows, o.picked};
+    if (const int e = launch_logits<T, SPLIT>(gemm_of(k, w, k.x, nv, p.rows, k.ld, 1, 0, 0), epi, st)) return e;
+  }
+  return 0;
 }
 
 template <int T, bool SPLIT, bool WIDE>

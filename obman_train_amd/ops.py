@@ -1001,7 +1001,7 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
     summation orders are fixed, so the same call gives the same bits.  The logits' gradient, of which dx and dw are sums, is rounded to 16-bit
     inputs' own type first (8 bits in bf16, 11 in fp16; db is summed before); in fp32 it has 22 bits.  In fp16 and fp32 it ends at 2^-39 and
     2^-51 of the largest row's weight (the loss's gradient, with ``"none"`` its largest entry): smaller probabilities give no gradient.  Rows
-    and classes up to 2^22, width up to 16384."""
+    and classes up to 2^22 each, width up to 16384; the forward pass's scratch takes 8 bytes for each row and 256 classes."""
     if reduction not in _REDUCTIONS:
         raise ValueError("reduction must be 'none', 'sum' or 'mean', got %r" % (reduction,))
     for name, t in (("x", x), ("weight", weight), ("target", target), ("bias", bias)):
