@@ -203,7 +203,8 @@ __device__ __forceinline__ void tile_of(const Gemm& g, int id, int& i, int& j, i
 struct Scale {
   const float* a;  // NULL = 1; else the power of two that operand was multiplied by
   const float* b;
-  __device__ __forceinline__ float inverse() const { return (a ? 1.f / *a : 1.f) * (b ? 1.f / *b : 1.f); }
+  // at most 2^127: two tensors near the end of fp32 would give an infinite factor, and 0 times that for a row of zeros
+  __device__ __forceinline__ float inverse() const { return fminf((a ? 1.f / *a : 1.f) * (b ? 1.f / *b : 1.f), 0x1p127f); }
 };
 
 struct Ctx {
@@ -1075,26 +1076,27 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish fx, Finish fw, Finis
   const int per = (width + 3) >> 2;
   const long total = f.rows * per;
   if ((long)blockIdx.x * 256 >= total) return;
-  const float k = alpha.value() * (f.scale ? 1.f / *f.scale : 1.f);
+  const float k = alpha.value(), k2 = f.scale ? 1.f / *f.scale : 1.f;  // (in turn: their product may end below the normal numbers, with few bits)
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
     const long r = i / per;
     const int c = (int)(i - r * per) * 4;
     const float* p = f.slabs + r * ld + c;
     f32x4 v = *reinterpret_cast<const f32x4*>(p);
     for (int s = 1; s < f.n; ++s) v += *reinterpret_cast<const f32x4*>(p + s * f.slab);
+    v = v * k * k2;
     const long at = r * width + c;
     if (c + 4 <= width) {
-      if (type == F32) *reinterpret_cast<f32x4u*>(static_cast<float*>(f.out) + at) = f32x4u{v[0] * k, v[1] * k, v[2] * k, v[3] * k};
+      if (type == F32) *reinterpret_cast<f32x4u*>(static_cast<float*>(f.out) + at) = f32x4u{v[0], v[1], v[2], v[3]};
       else {
         u16x4u o;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = type == BF16 ? narrow<BF16>(v[e] * k) : narrow<F16>(v[e] * k);
+        for (int e = 0; e < 4; ++e) o[e] = type == BF16 ? narrow<BF16>(v[e]) : narrow<F16>(v[e]);
         *reinterpret_cast<u16x4u*>(static_cast<u16*>(f.out) + at) = o;
       }
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (c + e < width) store_one(f.out, type, at + e, v[e] * k);
+        if (c + e < width) store_one(f.out, type, at + e, v[e]);
     }
   }
 }

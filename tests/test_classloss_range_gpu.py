@@ -150,3 +150,37 @@ def test_far_off_rows_in_pieces_and_from_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a.detach(), r) for a, r in zip(out, want[k % 2])), k
+
+
+@pytest.mark.parametrize("scale", [1e-34, 1e-30, 1e30])
+def test_means_of_operands_far_from_one(scale):
+    """Tiny features against a huge table and the other way round, averaged: what takes scales and average back together lies below fp32's normal
+    numbers.  dx and dw are right to their bounds as at ordinary sizes."""
+    from obman_train_amd import ops
+
+    for rows, classes, width in ((90, 130, 40), (3001, 400, 24)):
+        x, w, t, _ = _case(rows, classes, width, torch.float32)
+        leaves = [v.requires_grad_() for v in (x * scale, w / scale)]
+        dx, dw = torch.autograd.grad(ops.linear_cross_entropy(leaves[0], leaves[1], t), leaves)
+        _, lse, g, rx, rw, _, xe, we, c, p = _exact(leaves[0], leaves[1], t, None, "mean")
+        dg = 2.0 ** -21 * g.abs() + 4 * _logit_bound(xe, we, lse)[:, None] * p / rows + 2.0 ** -50 / rows
+        sums = lambda n: (n / 8 + 8) * 2.0 ** -24 + 2.0 ** -20  # noqa: E731
+        bx, bw = dg @ we.abs() + sums(classes) * (g.abs() @ we.abs()), dg.t() @ xe.abs() + sums(rows) * (g.abs().t() @ xe.abs())
+        smallest = 2.0 ** -149  # fp32's last step, where a gradient of 1e-34 over 3 001 rows ends
+        assert ((dx.double() - rx).abs() <= bx + smallest).all(), float(((dx.double() - rx).abs() / bx).max())
+        assert ((dw.double() - rw).abs() <= bw + smallest).all(), float(((dw.double() - rw).abs() / bw).max())
+
+
+def test_rows_of_zeros_beside_operands_near_the_end_of_fp32():
+    """Features and table near 2^125: rows of zeros have the loss log V and finite gradients' rows, as any row of zeros."""
+    import math
+
+    from obman_train_amd import ops
+
+    x, w, t, _ = _case(90, 130, 40, torch.float32)
+    x[:-1] = 0.0
+    x[-1] *= 1e37
+    w *= 1e37
+    with torch.no_grad():
+        loss = ops.linear_cross_entropy(x, w, t, reduction="none")
+    assert float((loss[:-1] - math.log(130)).abs().max()) <= 8 * 2.0 ** -24 * math.log(130)
