@@ -6,6 +6,7 @@ in ``csrc/*.hip``.  Every op requires fp32 ROCm tensors and raises otherwise - n
 import ctypes as _ct
 
 import torch
+from torch.autograd import forward_ad as _fw
 
 from . import _lib
 
@@ -943,6 +944,12 @@ class _on_device:
 _SIZES = _ct.c_long * 3
 
 
+def _has_tangent(*tensors):
+    """Whether a tensor carries a forward-mode derivative: such a call goes to the autograd function, which refuses it (raw kernels would drop
+    the tangent without a word)."""
+    return getattr(_fw, "_current_level", 0) >= 0 and any(t is not None and _fw.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _class_loss_forward(x, weight, bias, target, ignore_index, reduction, keeps, need=(False, False, False)):
     """-> loss, and with ``keeps`` what the backward pass needs: its copies of the operands, the call's parameters, the size of its scratch.
     All scratch is of this call alone: recorded into a graph it is the graph's."""
@@ -997,7 +1004,7 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
     class is all below 2^-16 of the tensor's largest element, zeros aside, that call runs on the fp32 instruction, in 2.6 times the time); ``target`` [...] is int64 or int32.  A row whose target is
     ``ignore_index`` has loss 0 and gradient 0 and takes no part in any gradient, even if its features are not finite; if every row
     is ignored the mean is 0.  A target that is neither a class nor ``ignore_index`` makes the loss NaN.  A bias of -inf takes a class
-    out of the sum.  Gradients for ``x``, ``weight`` and ``bias`` (only those that need one are computed), once differentiable;
+    out of the sum.  Gradients for ``x``, ``weight`` and ``bias`` (only those that need one are computed), once differentiable, in reverse mode only;
     summation orders are fixed, so the same call gives the same bits.  The logits' gradient, of which dx and dw are sums, is rounded to 16-bit
     inputs' own type first (8 bits in bf16, 11 in fp16; db is summed before); in fp32 it has 22 bits.  In fp16 and fp32 it ends at 2^-39 and
     2^-51 of the largest row's weight (the loss's gradient, with ``"none"`` its largest entry): smaller probabilities give no gradient.  Rows
@@ -1026,6 +1033,6 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
         return x.float().sum(-1) + zero if reduction == "none" else zero
     x, weight, target = x.contiguous(), weight.contiguous(), target.contiguous()
     bias = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)) or _has_tangent(x, weight, bias):
         return _LinearCrossEntropy.apply(x, weight, bias, target, int(ignore_index), _REDUCTIONS[reduction])
     return _class_loss_forward(x, weight, bias, target, int(ignore_index), _REDUCTIONS[reduction], False)[0]
