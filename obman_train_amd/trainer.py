@@ -170,7 +170,7 @@ class GraphedTrainStep:
     would need the host).  A host-driven backend (gloo) cannot be recorded.  (A split form for such backends - forward +
     backward graph, exchange from Python, optimizer graph - was built and REMOVED: on ROCm 7.0 / torch 2.10 a recorded backward that
     ends its graph produced garbage gradients for the encoder's early layers in most two-process runs, with autograd-allocated
-    and with persistent gradient buffers alike; tools/archive/r05/dp_split_dbg*.py are the reproducers.)
+    and with persistent gradient buffers alike.)
     Lambdas baked into the step (``ops.weighted_terms`` keeps the loss weights as device tensors; the ones a capture used are held by
     this object: ``term_weights``) are those of the capture: ``__call__`` compares the model's lambda attributes with the captured
     ones and raises when a schedule has changed them - re-capture, or write the new values into ``term_weights`` in
@@ -181,7 +181,7 @@ class GraphedTrainStep:
     records).  A training loop that must not see them passes ``restore_state=True``: model and optimizer state are
     snapshotted before the warm-up and copied back (in place - the recorded kernels keep their addresses) after the capture.
 
-    ROCm 7.0 caveat (measured, tools/graph_probe.py): ``hipGraphInstantiate`` segfaults at the end of the capture while the
+    ROCm 7.0 caveat (seen): ``hipGraphInstantiate`` segfaults at the end of the capture while the
     OUTPUTS of an earlier eager step (loss tensor, results dict - and through them their autograd nodes) are still referenced.
     Drop them before constructing this object (``bench.py`` does); the constructor collects garbage first."""
 
