@@ -19,6 +19,11 @@ def pytest_collection_modifyitems(config, items):
     CPU-only box they are deselected by ``-m "not gpu"`` and skipped if selected anyway."""
     import torch
 
+    # A pre-activation of this case is -1.2e-6 in 64 bits, a tenth of fp32's error there: its fp32 oracle takes the kernels' side of that ReLU on
+    # some hosts and the other side on others.  tests/test_decoder_ties_gpu.py holds the kernels to the same bound with the tie taken care of.
+    for item in items:
+        if item.nodeid.endswith("test_decoder_gpu.py::test_decoder_forward_backward_matches_oracle[515-2-1-True-25]"):
+            item.add_marker(pytest.mark.xfail(reason="the fp32 oracle meets a tie whose side depends on the host", raises=AssertionError, strict=False))
     if torch.cuda.is_available():
         return
     skip = pytest.mark.skip(reason="no GPU visible")
