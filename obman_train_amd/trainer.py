@@ -145,6 +145,7 @@ def _lambda_signature(model):
 
 class GraphedTrainStep:
     """One training step (forward -> zero_grad -> backward -> optimizer.step) recorded ONCE into a hipGraph and replayed.
+    ``max_grad_norm`` is ``train_step``'s: the clipping is recorded with the step.
 
     Why: the step is ~1 000 kernel launches.  With fp32 convolutions the GPU needs 11 ms for them and the host 5 ms to enqueue
     them, so the host is idle half of the time; with the bf16 encoder the GPU needs 5.9 ms and the same 5 ms of enqueue leave
@@ -185,7 +186,7 @@ class GraphedTrainStep:
     OUTPUTS of an earlier eager step (loss tensor, results dict - and through them their autograd nodes) are still referenced.
     Drop them before constructing this object (``bench.py`` does); the constructor collects garbage first."""
 
-    def __init__(self, model, optimizer, sample, warmup=3, restore_state=False, buckets=None):
+    def __init__(self, model, optimizer, sample, warmup=3, restore_state=False, buckets=None, max_grad_norm=None):
         import copy
         import gc
 
@@ -212,7 +213,7 @@ class GraphedTrainStep:
         side.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(side):  # eager steps on the side stream: lazy initialisation, MIOpen find, allocator growth
             for _ in range(max(int(warmup), 1)):
-                train_step(model, optimizer, self.static, self.buckets)
+                train_step(model, optimizer, self.static, self.buckets, max_grad_norm=max_grad_norm)
         torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
         if self.buckets is not None and self.buckets.some_rank_lacked_a_gradient():
@@ -233,14 +234,14 @@ class GraphedTrainStep:
         self.graph = torch.cuda.CUDAGraph()
         if self.mode == "single":
             with torch.cuda.graph(self.graph):
-                self.total, self.results, self.losses = train_step(model, optimizer, self.static)
+                self.total, self.results, self.losses = train_step(model, optimizer, self.static, max_grad_norm=max_grad_norm)
         else:
             # thread_local: the process group's watchdog thread may touch the runtime while this thread records
             b = self.buckets
             b.capturing = True
             try:
                 with torch.cuda.graph(self.graph, capture_error_mode="thread_local"):
-                    self.total, self.results, self.losses = train_step(model, optimizer, self.static, b)
+                    self.total, self.results, self.losses = train_step(model, optimizer, self.static, b, max_grad_norm=max_grad_norm)
             finally:
                 b.capturing = False
         # the loss-weight tensors this capture took out of ops' cache: kept alive here; [(values, tensor)] (a key another, uncollected
