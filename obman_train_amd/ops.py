@@ -1001,7 +1001,8 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
 
     ``x``, ``weight`` and ``bias`` [classes] are fp32, bf16 or fp16, all of one type (products of 16-bit types run on the matrix
     cores as they are, fp32 ones as three fp16 products: an element is right to 2^-22 of its row's or class's largest; if a row of ``x`` or a
-    class is all below 2^-16 of the tensor's largest element, zeros aside, that call runs on the fp32 instruction, in 2.6 times the time); ``target`` [...] is int64 or int32.  A row whose target is
+    class is all below 2^-16 of the tensor's largest element, zeros aside, that call runs on the fp32 instruction, in 2.6 times the time); ``target`` [...] is int64 or int32.
+    In an autocast region operands of different types are taken in the region's, as ``F.linear`` takes them.  A row whose target is
     ``ignore_index`` has loss 0 and gradient 0 and takes no part in any gradient, even if its features are not finite; if every row
     is ignored the mean is 0.  A target that is neither a class nor ``ignore_index`` makes the loss NaN.  A bias of -inf takes a class
     out of the sum.  Gradients for ``x``, ``weight`` and ``bias`` (only those that need one are computed), once differentiable, in reverse mode only;
@@ -1018,6 +1019,9 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
             raise _lib.ObmanHipError("%s must be a ROCm device tensor (the HIP path has no CPU fallback)" % name)
         if t.get_device() != x.get_device():
             raise ValueError("x, weight, target and bias must be on one device, got %s and %s" % (x.device, t.device))
+    dtypes = {t.dtype for t in (x, weight, bias) if t is not None}
+    if len(dtypes) > 1 and dtypes <= _CLASS_TYPES.keys() and torch.is_autocast_enabled("cuda"):
+        x, weight, bias = (None if t is None else t.to(torch.get_autocast_dtype("cuda")) for t in (x, weight, bias))
     if x.dtype not in _CLASS_TYPES or weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
         raise TypeError("x, weight and bias must all be fp32, bf16 or fp16, got %s, %s, %s" % (x.dtype, weight.dtype, None if bias is None else bias.dtype))
     if target.dtype not in (torch.int64, torch.int32):
