@@ -199,6 +199,8 @@ class ObmanAdam(torch.optim.Adam):
             devices |= cache["devices"]
             work.append((cache["addr"], len(params), float(lr), float(b1), float(b2), float(group["eps"]), float(group["weight_decay"])))
         if not work:
+            if self.max_grad_norm is not None:  # no gradient at all: their norm is 0, not the step's before
+                self.grad_norm = torch.zeros((), device=self.param_groups[0]["params"][0].device)
             return loss
         if len(devices) > 1:
             if self.max_grad_norm is not None:
