@@ -689,32 +689,27 @@ __global__ __launch_bounds__(256) void absmax_kernel(const float* __restrict__ x
 
 // Every thread of the block: whether fp32 operands are kept in full, and the powers of two that bring the largest elements to 2^13 .. 2^14
 // (1 for an all-zero tensor, and in full)
-struct Scales { float scale[2]; bool full; };
+struct Scales { float x, w; bool full; };
+__device__ __forceinline__ float scale_to(float m) {
+  int e = 0;
+  if (m > 0.f) (void)frexpf(m, &e);  // m = f 2^e, f in [0.5, 1)
+  e = 14 - e;
+  e = e > 120 ? 120 : e < -112 ? -112 : e;  // a power of two and its inverse are normal numbers
+  return m > 0.f ? ldexpf(1.f, e) : 1.f;
+}
 __device__ Scales scales_of(const float* __restrict__ part) {
   __shared__ float red[4][4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float v[4][2];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float* p = part + k * MAX_PARTS + threadIdx.x;
-    const float m = k < 2 ? wave_max(fmaxf(p[0], p[256])) : -wave_max(-fminf(p[0], p[256]));
-    if (lane == 0) red[k][wave] = m;
-  }
+  for (int k = 0; k < 4; ++k) { v[k][0] = part[k * MAX_PARTS + threadIdx.x]; v[k][1] = part[k * MAX_PARTS + threadIdx.x + 256]; }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) red[k][threadIdx.x >> 6] = k < 2 ? wave_max(fmaxf(v[k][0], v[k][1])) : -wave_max(-fminf(v[k][0], v[k][1]));  // (64 lanes, one value)
   __syncthreads();
-  Scales o;
-  o.full = false;
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const float m = fmaxf(fmaxf(red[k][0], red[k][1]), fmaxf(red[k][2], red[k][3]));
-    const float least = fminf(fminf(red[2 + k][0], red[2 + k][1]), fminf(red[2 + k][2], red[2 + k][3]));
-    int e = 0;
-    if (m > 0.f) (void)frexpf(m, &e);  // m = f 2^e, f in [0.5, 1)
-    e = 14 - e;
-    e = e > 120 ? 120 : e < -112 ? -112 : e;  // a power of two and its inverse are normal numbers
-    o.scale[k] = m > 0.f ? ldexpf(1.f, e) : 1.f;
-    o.full |= m > 0.f && m * (1.f / SPREAD) > least;
-  }
-  if (o.full) o.scale[0] = o.scale[1] = 1.f;
-  return o;
+  const auto top = [&](int k) { return fmaxf(fmaxf(red[k][0], red[k][1]), fmaxf(red[k][2], red[k][3])); };
+  const auto least = [&](int k) { return fminf(fminf(red[k][0], red[k][1]), fminf(red[k][2], red[k][3])); };
+  const float x = top(0), w = top(1);
+  const bool full = (x > 0.f && x * (1.f / SPREAD) > least(2)) || (w > 0.f && w * (1.f / SPREAD) > least(3));
+  return full ? Scales{1.f, 1.f, true} : Scales{scale_to(x), scale_to(w), false};
 }
 
 // x (grid row 0) and w (1) into blocks of columns, [blocks][padded rows][32]: zeros behind the width, behind the last row and for
@@ -730,7 +725,7 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack px, Pack pw, int width, 
   bool full = false;
   if constexpr (TYPE == F32) {
     const Scales s = scales_of(part);
-    sc = s.scale[blockIdx.y];
+    sc = first ? s.x : s.w;
     full = s.full;
     if (blockIdx.x == 0 && threadIdx.x == 0) {
       scale[blockIdx.y] = sc;
@@ -741,9 +736,7 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack px, Pack pw, int width, 
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
     const long r = i / chunks;
     const int c = (int)(i - r * chunks) * 8;
-    u16 hi[8], lo[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) hi[e] = lo[e] = 0;
+    u32x4 one = {0, 0, 0, 0}, two = {0, 0, 0, 0};  // fp32: hi and lo, or in full the first four and the others
     if (r < p.rows && (!first || target_of(target, wide, r) != ignore)) {
       const long at = r * width + c;
       if constexpr (TYPE == F32) {
@@ -757,35 +750,34 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack px, Pack pw, int width, 
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = c + e < width ? q[e] : 0.f;
         }
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float y0 = v[e] * sc, y1 = v[e + 1] * sc;
+          const u16 h0 = narrow<F16>(y0), h1 = narrow<F16>(y1);
+          const u16 l0 = fabsf(y0) < INFINITY ? narrow<F16>(y0 - widen<F16>(h0)) : (u16)0, l1 = fabsf(y1) < INFINITY ? narrow<F16>(y1 - widen<F16>(h1)) : (u16)0;
+          one[e / 2] = h0 | (unsigned)h1 << 16;
+          two[e / 2] = l0 | (unsigned)l1 << 16;
+        }
         if (full) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {  // the eight in a row, two 16-bit halves each
-            hi[2 * e] = (u16)(__float_as_uint(v[e]) & 0xffffu), hi[2 * e + 1] = (u16)(__float_as_uint(v[e]) >> 16);
-            lo[2 * e] = (u16)(__float_as_uint(v[e + 4]) & 0xffffu), lo[2 * e + 1] = (u16)(__float_as_uint(v[e + 4]) >> 16);
-          }
-        } else
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float y = v[e] * sc;
-          hi[e] = narrow<F16>(y);
-          lo[e] = fabsf(y) < INFINITY ? narrow<F16>(y - widen<F16>(hi[e])) : (u16)0;
+          for (int e = 0; e < 4; ++e) { one[e] = __float_as_uint(v[e]); two[e] = __float_as_uint(v[e + 4]); }
         }
       } else {
         const u16* q = static_cast<const u16*>(p.src) + at;
         if (c + 8 <= width) {
           const u16x8u a = *reinterpret_cast<const u16x8u*>(q);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) hi[e] = a[e];
+          for (int e = 0; e < 8; ++e) one[e / 2] |= (unsigned)a[e] << (16 * (e & 1));
         } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) hi[e] = c + e < width ? q[e] : (u16)0;
+          for (int e = 0; e < 8; ++e) one[e / 2] |= (c + e < width ? (unsigned)q[e] : 0u) << (16 * (e & 1));
         }
       }
     }
     constexpr int K = Step<TYPE == F32>;
     u16* o = p.dst + ((long)(c / K) * p.padded + r) * 32 + (full ? 2 : 1) * (c % K);
-    *reinterpret_cast<u32x4*>(o) = *reinterpret_cast<u32x4*>(hi);
-    if constexpr (TYPE == F32) *reinterpret_cast<u32x4*>(o + (full ? 8 : 16)) = *reinterpret_cast<u32x4*>(lo);
+    *reinterpret_cast<u32x4*>(o) = one;
+    if constexpr (TYPE == F32) *reinterpret_cast<u32x4*>(o + (full ? 8 : 16)) = two;
   }
 }
 
