@@ -14,8 +14,9 @@
 // whole tensor ends at 2^-39 of its largest element, so this holds while every row's largest element (all zeros aside) is within
 // SPREAD = 2^16 of it: 2^-22 of the row's own.  The pass that finds the largest element finds that out too, on the device; if a row of x or
 // a class of w lies further off, the same kernels take the operands as fp32 and the fp32 instruction (FULL below; 19 200 x 16 050 x 512 forward and
-// backward: 9.6 ms against 3.7).  g has |g| <= max |c|: in fp16 it is scaled to 2^14.  Rounding g to 16 bits (its own
-// size, before sums of many rows or classes) costs as much again as rounding the result.  With fp32 operands g is hi + lo too, and its lo
+// backward: 9.6 ms against 3.7).  g has |g| <= max |c|: in fp16 it is scaled to 2^14.  Rounding g to the inputs' 16 bits (its own
+// size, before sums of many rows or classes) adds a quarter to the error that rounding the result makes: 2-norms of dx and dw 2.05e-3 off for 1.66e-3 in
+// bf16, 2.56e-4 for 2.07e-4 in fp16; a second plane would cost two products more of four.  With fp32 operands g is hi + lo too, and its lo
 // is kept 2^12 times as large (the factor comes out of the other operand's hi): g is mostly probabilities, whose small ones are what a class
 // that is never a label learns from, and so its bits end at 2^-51 of max |c| instead of 2^-39.
 //
@@ -525,10 +526,11 @@ struct SlabStore {
 };
 
 // C[i, j] = sum_k A(i, k) B(j, k)
-// Bound: power.  At 19 200 x 64 050 x 512 in bf16 the forward product takes 1.36 ms (925 Tflop/s), g 1.49, dx and dw together 2.39
-// (1055); the matrix pipe is busy 56 - 57 % of cycles whose clock the chip holds at 1.6 - 1.75 GHz.  (Taking a fifth of the cycles out of
-// the forward product, by the blocked operands, the epilogue and the order of reads and loads, took 6 % off its time.)  fp32 at
-// 19 200 x 16 050 x 512: 70 % at 1.5 - 1.7 GHz, 1080 - 1220 Tflop/s of fp16 products.  A library's large bf16 product reaches 1375 here.
+// Bound: the matrix pipe waits.  At 19 200 x 64 050 x 512 in bf16 the forward product takes 1.21 - 1.37 ms (920 - 1040 Tflop/s) with the pipe busy 55 % of
+// cycles at 1.81 GHz, dx and dw of a piece 0.46 ms, 55 % at 1.89; a library's 8192^3 product on the same card has it busy 87 % at 1.59 GHz (1460 Tflop/s under
+// the profiler).  The clock falls as the pipe fills: busy share times clock is 1.00 here and 1.39 there.  LDS is read in 14 - 22 % of cycles, without
+// conflicts; a step's twelve fragment reads stand before its first product, with one other wave on the SIMD to cover them.  fp32 at 19 200 x 16 050 x 512:
+// 70 % at 1.68 GHz.  (Counters: profiles/training_tail_kernel_stats.md.)
 // G: which operand is g (its lo is G_LO times as large)
 enum { G_NONE, G_A, G_B };
 __device__ __forceinline__ u32x4 lowered(u32x4 hi) { return __builtin_bit_cast(u32x4, __builtin_bit_cast(f16x8, hi) * (_Float16)(1.f / G_LO)); }
@@ -785,7 +787,7 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack px, Pack pw, int width, 
 // its lanes load 16 bytes of each of the 32 class rows straight into matrix operands (a lane's element order along the width is free
 // as long as x, staged in LDS, has the same), fp32 on the fp32 instruction.  Blocks run over the table with running statistics; a
 // second launch joins them (one block for everything is 3 us quicker up to 2^17 elements of the table and loses soon behind: left out).
-// One row against 64 050 x 512 in bf16: 13 us, 5.0 TB/s (a large copy: 4.8).
+// One row against 64 050 x 512 in bf16: 17 us under the profiler, 3.9 TB/s, the 66 MB partly from the 256 MB cache (a large copy: 4.8).
 constexpr int FEW = 64;  // most rows: at 64 050 classes x 512 in bf16, 64 take 36 us here and 60 packed, 128 would take 70 and 62
 template <int TYPE> struct FewT { static constexpr int E = 8; };  // elements of a 16-byte piece
 template <> struct FewT<F32> { static constexpr int E = 4; };

@@ -83,7 +83,7 @@ def _norm_call(tensors, dev, types, norm_kind, max_norm=None):
 def grad_norm(tensors, norm_type=2.0):
     """The norm of all elements of all ``tensors`` (gradients, fp32 / bf16 / fp16, mixed) as one vector: a 0-dim fp32 tensor on
     their device, without a host synchronisation.  ``norm_type`` 2, 1 or inf.  Summed in 64 bits in a fixed order: bit-reproducible.
-    An empty list gives 0 (on the CPU); entries that are ``None`` (parameters without a gradient) are skipped."""
+    The result carries no derivative.  An empty list gives 0 (on the CPU); entries that are ``None`` (parameters without a gradient) are skipped."""
     kind = _norm_kind(norm_type)
     if isinstance(tensors, torch.Tensor):
         tensors = [tensors]
