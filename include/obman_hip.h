@@ -296,7 +296,7 @@ int obman_bf16_shadow(const float* src, uint16_t* dst, long n, obman_stream_t st
  * 2 fp16), at element alignment; target [rows] int64 (target_wide = 1) or int32.  Rows whose target is ignore_index count for
  * nothing, whatever their x holds; another target outside [0, classes) makes the row's loss and every gradient NaN.
  * An element of fp32 x or w is right to 2^-22 of its row's largest (pairs of fp16; the fp32 instruction where a row's largest element is
- * below 2^-16 of the tensor's, rows of zeros aside, which the device finds out).
+ * below 2^-16 of the tensor's, rows of zeros aside, which the device finds out), in tensors whose largest element is at least 2^-106.
  * reduction: 0 per row, 1 sum, 2 mean over the rows that are not ignored (0 if there are none).
  * rows, classes: at most 2^22 each; width: at most 16384; the forward scratch takes 8 bytes for each row and 256 classes.
  * Forward: loss (rows floats, or one).  keep holds what the backward pass needs - it does not read x and w again; NULL (keeps = 0

@@ -649,7 +649,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void grads_kernel(Gemm gx, Slab ex, 
 // of the kept rows of x (grid row 0) and of w (1): the largest finite |element|, and the least of the rows' largest (rows of zeros
 // aside).  MAX_PARTS block values each: [largest of x, of w, least of x, of w]
 constexpr int MAX_PARTS = 512;
-__device__ __forceinline__ float wave_max(float m) {  // within 16 lanes, then of the four 16s: a tenth of the time of six shuffles
+__device__ __forceinline__ float wave_max(float m) {  // within 16 lanes, then of the four 16s, all in registers
   m = fmaxf(m, obman_dpp<0xB1>(m));
   m = fmaxf(m, obman_dpp<0x4E>(m));
   m = fmaxf(m, obman_dpp<0x141>(m));
